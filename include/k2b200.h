@@ -42,10 +42,11 @@ typedef enum {
 
 /* Text of the last error on the calling thread. */
 const char *k2b200_last_error(void);
-/* ABI version of the library (bumped on any signature change or new entry point;
+/* ABI version of the library, bumped where a caller of the one before would break;
  * 3: pruned intersection, score derivatives, k2b200_upload_i32;
  * 4: k2b200_band_*;
- * 5: k2b200_peer_reduce_*, k2b200_loss_sum_all_reduce, zero_fill in k2b200_band_loss_args). */
+ * 5: k2b200_peer_reduce_*, k2b200_loss_sum_all_reduce, zero_fill in k2b200_band_loss_args
+ *    (k2b200_token_scores* and k2b200_distillation* came later and changed nothing else). */
 int32_t k2b200_abi_version(void);
 
 /* Benchmark bookkeeping (no counterpart in the reference's bindings; its
@@ -824,6 +825,83 @@ int32_t k2b200_loss_sum_all_reduce(const void *values, int32_t n, int32_t values
                                    int32_t poll_limit, double *out, void *stream,
                                    void *after_stream);
 int32_t k2b200_peer_reduce_status(void *local_buf, void *stream, int32_t *status);
+
+/* ---------------------------------------------------------------------------
+ * Scores of given classes, entropies and top classes of the rows that a network gives, and
+ * distillation from a teacher's top classes.  The reference has neither; they read the same
+ * rows as its callers' log_softmax (k2/python/k2/ctc_loss.py:28-208 takes its result).
+ *
+ * A row holds the scores x of C classes, log p_c = x_c - log sum exp x.  Of NaN and +inf among
+ * them comes NaN; a class of score -inf has p = 0, and where all have it, every log p is -inf.
+ * ------------------------------------------------------------------------- */
+typedef enum { K2B200_F32 = 0, K2B200_F16 = 1, K2B200_BF16 = 2 } k2b200_float_type;
+/* top_k of token scores, classes per row of a teacher */
+#define K2B200_MAX_TOP 128
+
+typedef struct {
+  const void *scores;     /* row (o, i) begins at o * outer_stride + i * inner_stride elements, */
+  int32_t type;           /* its classes are adjacent; k2b200_float_type */
+  int32_t num_classes;
+  int64_t outer, inner;   /* rows: outer * inner < 2^31 */
+  int64_t outer_stride, inner_stride;
+  const void *lengths;    /* [outer] or NULL: the row (o, i) counts where i < lengths[o]; rows that */
+  int32_t lengths_64;     /* do not count are not read.  int32, or int64 */
+} k2b200_class_rows;
+
+/* Where the upstream gradient of a value per row is: base + o * outer + i * inner elements. */
+typedef struct {
+  const float *grad;      /* NULL: none */
+  int64_t outer, inner, top; /* top: from one of the top classes to the next */
+} k2b200_row_grad;
+
+/* tokens [rows] (NULL: none are asked for): -1 has log-prob 0, any other that is no class NaN.
+ * log_probs, entropy [rows] (each may be NULL); top_log_probs, top_tokens [rows, top_k], largest
+ * first, a lower class before a higher one of the same score, NaN before all numbers.  A row that
+ * does not count gets log-probs and entropy 0 and top_tokens -1.  norm [rows, 4]: for the
+ * backward pass (NULL: none follows). */
+int32_t k2b200_token_scores(const k2b200_class_rows *rows, const void *tokens, int32_t tokens_64,
+                            int32_t top_k, float *log_probs, float *entropy,
+                            float *top_log_probs, int32_t *top_tokens, float *norm,
+                            void *stream);
+/* grad_scores: the gradient of the rows, of their type, its row (o, i) at o * grad_outer_stride +
+ * i * grad_inner_stride; every row of it is written, with zeros where a row does not count. */
+int32_t k2b200_token_scores_backward(const k2b200_class_rows *rows, const void *tokens,
+                                     int32_t tokens_64, int32_t top_k, const int32_t *top_tokens,
+                                     const float *norm, const k2b200_row_grad *log_probs_grad,
+                                     const k2b200_row_grad *entropy_grad,
+                                     const k2b200_row_grad *top_log_probs_grad,
+                                     void *grad_scores, int64_t grad_outer_stride,
+                                     int64_t grad_inner_stride, void *stream);
+
+typedef struct {
+  const void *tokens;     /* [rows, entries]: classes, -1 where a row has fewer; one that comes */
+  int32_t tokens_64;      /* twice counts twice; any other that is no class makes the row NaN */
+  const void *scores;     /* [rows, entries]: log-probs or logits t of those classes */
+  int32_t type;           /* k2b200_float_type */
+  int32_t entries;        /* 1 to K2B200_MAX_TOP */
+  float temperature;      /* > 0 */
+  float weight;
+  int32_t reduction;      /* 0: none, 1: sum, 2: mean over the rows that count */
+} k2b200_teacher;
+
+/* Per row weight * T^2 * sum_j q_j (log q_j - log p_j), with q = softmax(t / T) over the entries
+ * and p = softmax(x / T) over all classes.  A row without an entry of finite score gives 0.
+ * loss: [rows], or one value.  grad_scores (may be NULL): the gradient of the sum or mean,
+ * as in k2b200_token_scores_backward.  norm [rows, 4] (NULL: no backward pass follows).
+ * workspace: k2b200_distillation_workspace_bytes(); the backward pass reads it. */
+size_t k2b200_distillation_workspace_bytes(const k2b200_class_rows *rows);
+int32_t k2b200_distillation(const k2b200_class_rows *rows, const k2b200_teacher *teacher,
+                            float *loss, float *norm, void *grad_scores,
+                            int64_t grad_outer_stride, int64_t grad_inner_stride,
+                            void *workspace, size_t workspace_bytes, void *stream);
+/* upstream: of every row, or of the one value (strides 0).  unless_one != 0 (one value):
+ * grad_scores already holds the gradient for an upstream of 1 and is left alone if it is 1. */
+int32_t k2b200_distillation_backward(const k2b200_class_rows *rows, const k2b200_teacher *teacher,
+                                     const float *norm, const k2b200_row_grad *upstream,
+                                     int32_t unless_one, void *grad_scores,
+                                     int64_t grad_outer_stride, int64_t grad_inner_stride,
+                                     const void *workspace, size_t workspace_bytes,
+                                     void *stream);
 
 #ifdef __cplusplus
 }

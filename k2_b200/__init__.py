@@ -3,6 +3,8 @@ loss path, behind k2's own Python API names for that path."""
 from . import _lib  # noqa: F401  (fails loudly when the CUDA library is missing)
 from .autograd import (dense_loss_supported, index_select, intersect_dense,  # noqa: F401
                        intersect_dense_pruned, intersect_dense_tot_scores)
+from .class_scores import (DistillationLoss, TokenLogProbs, distillation_loss,  # noqa: F401
+                           token_log_probs)
 from .ctc_loss import CtcLoss, ctc_loss  # noqa: F401
 from .decode import get_aux_labels, get_lattice, one_best_decoding  # noqa: F401
 from .dense_fsa_vec import DenseFsaVec  # noqa: F401

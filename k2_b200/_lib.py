@@ -110,6 +110,25 @@ class OnlineArgs(ctypes.Structure):
     ]
 
 
+class ClassRows(ctypes.Structure):
+    _fields_ = [
+        ("scores", c_vp), ("type", c_i32), ("num_classes", c_i32), ("outer", c_i64),
+        ("inner", c_i64), ("outer_stride", c_i64), ("inner_stride", c_i64), ("lengths", c_vp),
+        ("lengths_64", c_i32),
+    ]
+
+
+class RowGrad(ctypes.Structure):
+    _fields_ = [("grad", c_vp), ("outer", c_i64), ("inner", c_i64), ("top", c_i64)]
+
+
+class Teacher(ctypes.Structure):
+    _fields_ = [
+        ("tokens", c_vp), ("tokens_64", c_i32), ("scores", c_vp), ("type", c_i32),
+        ("entries", c_i32), ("temperature", c_f32), ("weight", c_f32), ("reduction", c_i32),
+    ]
+
+
 class FsaView(ctypes.Structure):
     _fields_ = [
         ("num_fsas", c_i32), ("num_states", c_i32), ("num_arcs", c_i32),
@@ -270,6 +289,19 @@ _sig("k2b200_loss_sum_all_reduce", c_i32,
       ctypes.c_uint64, c_i32, c_vp, c_vp, c_vp])
 _sig("k2b200_peer_reduce_status", c_i32, [c_vp, c_vp, ctypes.POINTER(c_i32)])
 
+_sig("k2b200_token_scores", c_i32,
+     [ctypes.POINTER(ClassRows), c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp])
+_sig("k2b200_token_scores_backward", c_i32,
+     [ctypes.POINTER(ClassRows), c_vp, c_i32, c_i32, c_vp, c_vp, ctypes.POINTER(RowGrad),
+      ctypes.POINTER(RowGrad), ctypes.POINTER(RowGrad), c_vp, c_i64, c_i64, c_vp])
+_sig("k2b200_distillation_workspace_bytes", c_sz, [ctypes.POINTER(ClassRows)])
+_sig("k2b200_distillation", c_i32,
+     [ctypes.POINTER(ClassRows), ctypes.POINTER(Teacher), c_vp, c_vp, c_vp, c_i64, c_i64, c_vp,
+      c_sz, c_vp])
+_sig("k2b200_distillation_backward", c_i32,
+     [ctypes.POINTER(ClassRows), ctypes.POINTER(Teacher), c_vp, ctypes.POINTER(RowGrad), c_i32,
+      c_vp, c_i64, c_i64, c_vp, c_sz, c_vp])
+
 EXPORTED = [
     "k2b200_last_error", "k2b200_abi_version", "k2b200_kernel_launch_count",
     "k2b200_profile_enable", "k2b200_profile_kernel", "k2b200_profile_read_ms", "k2b200_row_splits_to_row_ids",
@@ -307,6 +339,8 @@ EXPORTED = [
     "k2b200_band_loss_backward", "k2b200_band_loss_status", "k2b200_band_loss_plan",
     "k2b200_band_loss_forward_reduce", "k2b200_band_loss_backward_dense",
     "k2b200_debug_set_copy_wait_limit",
+    "k2b200_token_scores", "k2b200_token_scores_backward",
+    "k2b200_distillation_workspace_bytes", "k2b200_distillation", "k2b200_distillation_backward",
 ]
 
 

@@ -38,7 +38,7 @@ def _stale() -> bool:
 
 
 HOST_PATH = os.path.join(_HERE, "_host.so")
-HOST_SOURCE = os.path.join(CSRC, "host", "torch_host.cc")
+HOST_SOURCES = [os.path.join(CSRC, "host", name) for name in ("torch_host.cc", "class_rows.cc")]
 
 
 # what _host.so was built for: it works with that Python and that torch only
@@ -63,7 +63,7 @@ def _host_stale(command) -> bool:
 
 
 def _host_command():
-    """The C++ compiler on the one translation unit that includes torch's headers;
+    """The C++ compiler on the translation units that include torch's headers;
     libk2b200.so is found next to it, torch's libraries are loaded by `import torch`."""
     import torch
     torch_dir = os.path.dirname(torch.__file__)
@@ -75,7 +75,7 @@ def _host_command():
             "-DTORCH_EXTENSION_NAME=_host",
             "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
             "-isystem", os.path.join(cuda, "include"),
-            "-isystem", sysconfig.get_paths()["include"], HOST_SOURCE, "-o", HOST_PATH,
+            "-isystem", sysconfig.get_paths()["include"], *HOST_SOURCES, "-o", HOST_PATH,
             "-L" + _HERE, "-l:libk2b200.so", "-Wl,-rpath,$ORIGIN",
             "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
             "-ltorch_cuda", "-ltorch", "-ltorch_python"]

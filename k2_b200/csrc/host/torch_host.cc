@@ -11,7 +11,6 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <pybind11/numpy.h>
 #include <torch/extension.h>
@@ -23,6 +22,8 @@
 #include <vector>
 
 #include "../../../include/k2b200.h"
+#include "class_rows.h"
+#include "node_name.h"
 #include "python_ints.h"
 
 namespace py = pybind11;
@@ -328,20 +329,6 @@ std::shared_ptr<BandLossNode> NewNode(int32_t mode) {
   return std::shared_ptr<BandLossNode>(node, torch::autograd::deleteNode);
 }
 
-template <typename T>
-void NameNode(const char *name) {
-  using namespace torch::autograd;  // the properties below are named without it
-  static PyTypeObject type;
-  static PyMethodDef methods[] = {
-      {"register_hook", THPCppFunction_register_hook, METH_O, nullptr},
-      {"register_prehook", THPCppFunction_register_prehook, METH_O, nullptr},
-      {"name", THPCppFunction_name, METH_NOARGS, nullptr},
-      {nullptr}};
-  static PyGetSetDef properties[] = {THP_FUNCTION_DEFAULT_PROPERTIES, {nullptr}};
-  _initFunctionPyTypeObject(type, name, properties, methods);
-  registerCppFunction(typeid(T), &type);
-}
-
 int32_t LensType(const at::Tensor &t) {
   switch (t.scalar_type()) {
     case at::kInt: return 1;
@@ -502,4 +489,5 @@ PYBIND11_MODULE(_host, m) {
   m.def("dense_layout", &DenseLayout);
   m.def("band_loss", &BandLoss);
   m.def("release_workspaces", &ReleaseWorkspaces);
+  BindClassRows(m);
 }
