@@ -841,8 +841,8 @@ typedef enum { K2B200_F32 = 0, K2B200_F16 = 1, K2B200_BF16 = 2 } k2b200_float_ty
 typedef struct {
   const void *scores;     /* row (o, i) begins at o * outer_stride + i * inner_stride elements, */
   int32_t type;           /* its classes are adjacent; k2b200_float_type */
-  int32_t num_classes;
-  int64_t outer, inner;   /* rows: outer * inner < 2^31 */
+  int32_t num_classes;    /* 1 to 2^30 */
+  int64_t outer, inner;   /* rows: outer * inner < 2^28 */
   int64_t outer_stride, inner_stride;
   const void *lengths;    /* [outer] or NULL: the row (o, i) counts where i < lengths[o]; rows that */
   int32_t lengths_64;     /* do not count are not read.  int32, or int64 */

@@ -1,7 +1,20 @@
-// Rows of class scores as the kernels of token_scores.cu and distillation.cu read them.
+// Rows of class scores as the kernels of token_scores.cu and distillation.cu hold them.
+//
+// A row is read once, as aligned vectors of 16 bytes, into the registers of a team of threads: a
+// warp up to 4 KB, 128 threads up to 16, 256 up to 64, and a cluster of up to 8 such blocks up to
+// 512.  Where the row begins inside a vector (any alignment of an element will do) the elements of
+// the first and the last vector are read one by one, and what lies outside the row is -inf there.
+// What a kernel needs of the row more than once it takes from the registers.  Longer rows are read
+// again, tile by tile.
+//
+//   p_c = 2^((x_c - high) * log2 e) / sum   high the largest score, sum over all classes
+//
+// Everything is computed in 32 bits, whatever the type of the scores.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "../../include/k2b200.h"
 #include "common.cuh"
@@ -9,13 +22,16 @@
 namespace k2b {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// (columns of a vector stay within 32 bits)
+constexpr int32_t kMaxClasses = 1 << 30;
 
 // What a kernel needs of k2b200_class_rows.
 template <typename T>
 struct Rows {
   const T *scores;
-  int32_t classes;
-  int64_t inner, outer_stride, inner_stride;
+  int32_t classes, count;
+  uint32_t inner;
+  int64_t outer_stride, inner_stride;
   const void *lengths;
   int32_t lengths_64;
 };
@@ -34,13 +50,16 @@ __device__ __forceinline__ int64_t IntAt(const void *ints, int32_t is_64, int64_
 template <typename T>
 __device__ __forceinline__ RowPlace PlaceOf(const Rows<T> &rows, int32_t r) {
   RowPlace p;
-  const uint32_t inner = (uint32_t)rows.inner, o = (uint32_t)r / inner;
+  const uint32_t o = (uint32_t)r / rows.inner;
   p.o = o;
-  p.i = (uint32_t)r - o * inner;
+  p.i = (uint32_t)r - o * rows.inner;
   p.counts = rows.lengths == nullptr || p.i < IntAt(rows.lengths, rows.lengths_64, p.o);
   return p;
 }
 
+// ---------------------------------------------------------------------------
+// numbers
+// ---------------------------------------------------------------------------
 __device__ __forceinline__ float ToFloat(float v) { return v; }
 __device__ __forceinline__ float ToFloat(__half v) { return __half2float(v); }
 __device__ __forceinline__ float ToFloat(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -69,45 +88,342 @@ __device__ __forceinline__ uint32_t OrderOf(float v) {
   if (v != v) return 0xffffffffu;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float ScoreOf(uint32_t order) {
+  return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
 __device__ __forceinline__ uint64_t KeyOf(float v, int32_t c) {
   return (uint64_t)OrderOf(v) << 32 | (uint32_t)~c;
 }
 
-__device__ __forceinline__ float TeamMax(float v) {
+// ---------------------------------------------------------------------------
+// vectors of 16 bytes
+// ---------------------------------------------------------------------------
+template <typename T>
+constexpr int kPer = 16 / (int)sizeof(T);
+
+__device__ __forceinline__ void Unpack(uint4 v, float (&f)[4], const float *) {
+  f[0] = __uint_as_float(v.x);
+  f[1] = __uint_as_float(v.y);
+  f[2] = __uint_as_float(v.z);
+  f[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void Unpack(uint4 v, float (&f)[8], const __nv_bfloat16 *) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+  for (int k = 0; k < 4; ++k) {
+    f[2 * k] = __uint_as_float(w[k] << 16);
+    f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void Unpack(uint4 v, float (&f)[8], const __half *) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+    f[2 * k] = p.x;
+    f[2 * k + 1] = p.y;
+  }
+}
+__device__ __forceinline__ uint4 Pack(const float (&f)[4], const float *) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                    __float_as_uint(f[3]));
+}
+template <typename Pair, Pair (*kRound)(float, float)>
+__device__ __forceinline__ uint4 PackPairs(const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const Pair p = kRound(f[2 * k], f[2 * k + 1]);
+    memcpy(&w[k], &p, 4);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 Pack(const float (&f)[8], const __half *) {
+  return PackPairs<__half2, __floats2half2_rn>(f);
+}
+__device__ __forceinline__ uint4 Pack(const float (&f)[8], const __nv_bfloat16 *) {
+  return PackPairs<__nv_bfloat162, __floats2bfloat162_rn>(f);
+}
+
+// Makes the compiler forget where a vector's words come from: it would keep a row unpacked between
+// the passes over it, in twice the registers.
+__device__ __forceinline__ uint4 &Packed(uint4 &v) {
+  asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w));
   return v;
 }
-__device__ __forceinline__ float TeamSum(float v) {
+// ... and does not unpack it before `sum` is what it is here: it would unpack all of a row's vectors
+// at once otherwise.
+__device__ __forceinline__ void After(uint4 &v, float &sum) {
+  asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w), "+f"(sum));
+}
+
+// The largest of a vector's scores; NaN are passed over.
+__device__ __forceinline__ float VectorMax(uint4 v, const float *) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+               fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+template <typename Pair>
+__device__ __forceinline__ Pair PairMax(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  Pair p[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) memcpy(&p[k], &w[k], 4);
+  return __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+}
+__device__ __forceinline__ float VectorMax(uint4 v, const __half *) {
+  const float2 f = __half22float2(PairMax<__half2>(v));
+  return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ float VectorMax(uint4 v, const __nv_bfloat16 *) {
+  const float2 f = __bfloat1622float2(PairMax<__nv_bfloat162>(v));
+  return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ uint4 LowestVector(const float *) {
+  return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+}
+__device__ __forceinline__ uint4 LowestVector(const __half *) {
+  return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+}
+__device__ __forceinline__ uint4 LowestVector(const __nv_bfloat16 *) {
+  return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+}
+
+// A row as aligned vectors: vector j holds the classes from Column(j) on, of which the first
+// vector's first `shift` and the last one's last are none of the row's.
+template <typename T>
+struct RowSpan {
+  const T *row;
+  int32_t classes, shift, vectors;
+  __device__ __forceinline__ RowSpan(const T *x, int32_t c) : row(x), classes(c) {
+    shift = (int32_t)(((uintptr_t)x & 15) / sizeof(T));
+    vectors = (shift + c + kPer<T> - 1) / kPer<T>;
+  }
+  __device__ __forceinline__ int32_t Column(int32_t j) const { return j * kPer<T> - shift; }
+  __device__ __forceinline__ bool Whole(int32_t c0) const {
+    return c0 >= 0 && c0 + kPer<T> <= classes;
+  }
+  // A vector that is not whole, element by element.
+  __device__ __forceinline__ uint4 Edge(int32_t j) const {
+    const int32_t c0 = Column(j);
+    float f[kPer<T>];
+#pragma unroll
+    for (int k = 0; k < kPer<T>; ++k) {
+      const int32_t c = c0 + k;
+      f[k] = c >= 0 && c < classes ? ToFloat(row[c]) : -INFINITY;
+    }
+    return Packed(f);  // (exact)
+  }
+  __device__ __forceinline__ uint4 Vector(int32_t j) const {
+    const int32_t c0 = Column(j);
+    return Whole(c0) ? *reinterpret_cast<const uint4 *>(row + c0) : Edge(j);
+  }
+  __device__ __forceinline__ static uint4 Packed(const float (&f)[kPer<T>]) {
+    uint4 v = Pack(f, static_cast<const T *>(nullptr));
+    return k2b::Packed(v);
+  }
+};
+
+// Vectors tile + i * kTeam + tid for i < kVectors of those before `last`.
+template <int kTeam, int kVectors, typename T>
+__device__ __forceinline__ void LoadTile(uint4 (&v)[kVectors], const RowSpan<T> &span,
+                                         int32_t tile, int32_t last, int32_t tid) {
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const int32_t j = tile + i * kTeam + tid, c0 = span.Column(j);
+    v[i] = j < last && span.Whole(c0) ? *reinterpret_cast<const uint4 *>(span.row + c0)
+                                      : LowestVector(span.row);
+  }
+  // the row's first and last vector: two threads of the team at most, in one step of a warp
+  // unless one thread has both
+  const int32_t end = span.vectors - 1;
+  int32_t edge = tile == 0 && tid == 0 && !span.Whole(span.Column(0)) ? 0 : -1;
+  int32_t more = end > 0 && end >= tile && end < min(last, tile + kTeam * kVectors) &&
+                         ((end - tile) & (kTeam - 1)) == tid && !span.Whole(span.Column(end))
+                     ? end
+                     : -1;
+  if (edge < 0) {
+    edge = more;
+    more = -1;
+  }
+  while (edge >= 0) {
+    const uint4 e = span.Edge(edge);
+    const int32_t slot = (edge - tile) / kTeam;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (i == slot) v[i] = e;
+    edge = more;
+    more = -1;
+  }
+}
+
+// Values for the classes of vector j into another row of the same length; `aligned`: both rows
+// begin at the same place of a vector.
+template <typename T>
+__device__ __forceinline__ void Store(T *out, const RowSpan<T> &span, bool aligned, int32_t j,
+                                      const float (&f)[kPer<T>]) {
+  const int32_t c0 = span.Column(j);
+  if (aligned && span.Whole(c0)) {
+    *reinterpret_cast<uint4 *>(out + c0) = Pack(f, out);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < kPer<T>; ++k)
+    if (c0 + k >= 0 && c0 + k < span.classes) out[c0 + k] = FromFloat<T>(f[k]);
+}
+
+// ---------------------------------------------------------------------------
+// teams
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float WarpMaxF(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ float WarpSumF(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-__device__ __forceinline__ uint64_t TeamMax(uint64_t v) {
+// Both sums at once: the halves of the warp take one each.
+__device__ __forceinline__ float2 WarpSum2F(float a, float b) {
+  const bool high = threadIdx.x & 16;
+  float mine = high ? b : a;
+  mine += __shfl_xor_sync(0xffffffffu, high ? a : b, 16);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, v, d);
-    v = o > v ? o : v;
+  for (int d = 8; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  const float other = __shfl_xor_sync(0xffffffffu, mine, 16);
+  return high ? make_float2(other, mine) : make_float2(mine, other);
+}
+
+// Blocks of an SM that a kernel is compiled for: the registers are the row's and some 40 more.
+constexpr int MinBlocks(int team, int vectors) {
+  return (vectors >= 16 ? 2 : vectors >= 8 ? 3 : 4) * (team == 128 ? 2 : 1);
+}
+
+template <int kTeam>
+__device__ __forceinline__ void TeamSync() {
+  if (kTeam == 32) __syncwarp(); else __syncthreads();
+}
+
+// This block's place in its cluster (0 of 1 without one).
+__device__ __forceinline__ uint32_t ClusterRank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t ClusterSize() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+// All threads of all blocks of the cluster; what was written to shared memory before is seen
+// behind it.
+__device__ __forceinline__ void ClusterSync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
+               ::: "memory");
+}
+// A shared variable of this block, in block `rank` of the cluster.
+template <typename V>
+__device__ __forceinline__ V ReadFrom(const V *mine, uint32_t rank) {
+  static_assert(sizeof(V) == 4 || sizeof(V) == 8, "4 or 8 bytes");
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(mine);
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+  V v;
+  if (sizeof(V) == 4) {
+    uint32_t w;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(there) : "memory");
+    memcpy(&v, &w, 4);
+  } else {
+    uint64_t w;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(w) : "r"(there) : "memory");
+    memcpy(&v, &w, 8);
   }
   return v;
 }
 
-// A row's scores are turned into p_c = 2^((x_c - high) * scale) / sum: high the largest (0 where
-// all are -inf), sum 0 where all are -inf.
-struct RowNorm {
-  float high, sum;
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+// How the rows of a call are dealt out.
+struct RowPlan {
+  int32_t team;     // threads per row and block: 32, 128, 256
+  int32_t vectors;  // per thread
+  int32_t cluster;  // blocks per row
+  bool again;       // the row does not fit and is read again
+  int32_t block;    // threads of a block: `team`, or several warps that are a team each
+  int32_t rows_per_block;
 };
+
+template <typename T>
+static inline RowPlan PlanRows(const Rows<T> &r) {
+  RowPlan p = {32, 1, 1, false, 32, 1};
+  const int64_t rows = r.count, size = sizeof(T);
+  // its vectors: one more where it does not begin with one
+  const bool whole = ((uintptr_t)r.scores | (uint64_t)(r.outer_stride * size) |
+                      (uint64_t)(r.inner_stride * size)) % 16 == 0;
+  const int64_t bytes = r.classes * size + (whole ? 0 : 16 - size);
+  const int32_t sms = NumSms();
+  if (bytes <= 32 * 8 * 16) {
+    while (bytes > 32 * 16 * p.vectors) p.vectors *= 2;
+    // few rows: a warp to an SM; many: eight rows to a block
+    p.rows_per_block = (int32_t)std::min<int64_t>(8, std::max<int64_t>(1, rows / sms));
+    p.block = 32 * p.rows_per_block;
+    return p;
+  }
+  p.team = p.block = bytes <= 128 * 8 * 16 ? 128 : 256;
+  if (p.team == 128) {
+    p.vectors = bytes <= 128 * 4 * 16 ? 4 : 8;
+    return p;
+  }
+  while (p.cluster < 8 && bytes > (int64_t)p.cluster * 256 * 16 * 16) p.cluster *= 2;
+  // few rows: over more SMs, down to 8 KB of the row each
+  while (p.cluster < 8 && rows * p.cluster * 2 <= sms && bytes > (int64_t)p.cluster * 2 * 8192)
+    p.cluster *= 2;
+  p.vectors = 4;
+  while (p.vectors < 16 && bytes > (int64_t)p.cluster * 256 * 16 * p.vectors) p.vectors *= 2;
+  p.again = bytes > (int64_t)p.cluster * 256 * 16 * p.vectors;
+  return p;
+}
+
+// A launch of `blocks` blocks in clusters; `behind`: see LaunchBehind (common.cuh).
+template <typename... Params, typename... Args>
+static cudaError_t LaunchRows(void (*kernel)(Params...), int64_t blocks, int32_t threads,
+                              size_t smem, int32_t cluster, bool behind, cudaStream_t stream,
+                              Args &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((uint32_t)blocks);
+  cfg.blockDim = dim3((uint32_t)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (uint32_t)cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (behind) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = attr;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
 
 // What the entry points ask of a k2b200_class_rows.
 static inline int32_t CheckRows(const k2b200_class_rows *rows) {
   K2B_REQUIRE(rows != nullptr, "NULL pointer");
   K2B_REQUIRE(rows->type >= K2B200_F32 && rows->type <= K2B200_BF16, "unknown type %d",
               rows->type);
-  K2B_REQUIRE(rows->num_classes > 0, "rows of no class");
-  K2B_REQUIRE(rows->outer >= 0 && rows->inner >= 0 && rows->outer < ((int64_t)1 << 31) &&
-                  rows->inner < ((int64_t)1 << 31) &&
-                  rows->outer * rows->inner < ((int64_t)1 << 31),
-              "%lld x %lld rows are more than fit", (long long)rows->outer,
+  K2B_REQUIRE(rows->num_classes > 0 && rows->num_classes <= kMaxClasses,
+              "rows of %d classes: 1 to 2^30", rows->num_classes);
+  // (blocks of a cluster count too: 8 to a row at most)
+  K2B_REQUIRE(rows->outer >= 0 && rows->inner >= 0 && rows->outer < ((int64_t)1 << 28) &&
+                  rows->inner < ((int64_t)1 << 28) &&
+                  rows->outer * rows->inner < ((int64_t)1 << 28),
+              "%lld x %lld rows: fewer than 2^28", (long long)rows->outer,
               (long long)rows->inner);
   K2B_REQUIRE(rows->scores != nullptr || rows->outer * rows->inner == 0, "NULL pointer");
   return kOk;
@@ -118,7 +434,8 @@ static inline Rows<T> RowsOf(const k2b200_class_rows *rows) {
   Rows<T> r;
   r.scores = static_cast<const T *>(rows->scores);
   r.classes = rows->num_classes;
-  r.inner = rows->inner;
+  r.count = (int32_t)(rows->outer * rows->inner);
+  r.inner = (uint32_t)rows->inner;
   r.outer_stride = rows->outer_stride;
   r.inner_stride = rows->inner_stride;
   r.lengths = rows->lengths;

@@ -1,18 +1,27 @@
 // Divergence of rows of scores from a teacher's distribution over its top classes, and its
 // gradient.
+//
+// With q = softmax(t / T) over a row's entries and p = softmax(x / T) over its classes, the loss is
+// T^2 sum_j q_j (log q_j - log p_j) and its gradient T (p_c - sum_j q_j [c = j]).  Distil holds the
+// row in registers (class_rows.cuh), so that loss and gradient take one read and one write of it;
+// the gradient is for an upstream of 1, and DistilBackward makes it again for another one.  All
+// classes are written as if the teacher had named none, whole vectors at a time, and its classes
+// again behind them.
 #include "class_rows.cuh"
 
 namespace k2b {
 
-constexpr int kDistilThreads = 128;
-
-// The workspace: what the row's gradient is multiplied with (weight, or weight / rows that count),
-// and the rows' losses.
+// What a row's loss and gradient are multiplied with: weight, or weight / rows that count.
 struct DistilScale {
   double exact;
   float rounded;
 };
-constexpr size_t kDistilHead = 256;
+// Known to the host, or to the device (a kernel before this one counts the rows).
+struct DistilBy {
+  const DistilScale *device;
+  DistilScale host;
+};
+constexpr size_t kDistilHead = 256;  // of the workspace; the blocks' losses follow
 
 struct Teacher {
   const void *tokens, *scores;
@@ -26,148 +35,367 @@ __device__ __forceinline__ float TeacherScore(const Teacher &t, int64_t k) {
                                 : __bfloat162float(static_cast<const __nv_bfloat16 *>(t.scores)[k]);
 }
 
+// Rows that count, of given lengths.  The kernel behind it starts meanwhile.
 __global__ void __launch_bounds__(1024)
-DistilScaleOf(const void *lengths, int32_t lengths_64, int64_t outer, int64_t inner, double weight,
-              int32_t mean, DistilScale *scale) {
+DistilCount(const void *lengths, int32_t lengths_64, int64_t outer, int64_t inner, double weight,
+            DistilScale *scale) {
+  LetNextStart();
   __shared__ long long counted;
   if (threadIdx.x == 0) counted = 0;
   __syncthreads();
   long long mine = 0;
-  if (mean && lengths)
-    for (int64_t o = threadIdx.x; o < outer; o += 1024) {
-      const int64_t n = IntAt(lengths, lengths_64, o);
-      mine += n < 0 ? 0 : n > inner ? inner : n;
-    }
-  atomicAdd(reinterpret_cast<unsigned long long *>(&counted), (unsigned long long)mine);
+  for (int64_t o = threadIdx.x; o < outer; o += 1024) {
+    const int64_t n = IntAt(lengths, lengths_64, o);
+    mine += n < 0 ? 0 : n > inner ? inner : n;
+  }
+  if (mine) atomicAdd(reinterpret_cast<unsigned long long *>(&counted), (unsigned long long)mine);
   __syncthreads();
   if (threadIdx.x == 0) {
-    const long long n = !mean ? 1 : lengths ? counted : outer * inner;
-    scale->exact = weight / (double)(n > 1 ? n : 1);
+    scale->exact = weight / (double)(counted > 1 ? counted : 1);
     scale->rounded = (float)scale->exact;
   }
 }
 
-__device__ __forceinline__ float DistilMax(float v, float *smem) {
-  v = TeamMax(v);
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = smem[0];
-  for (int w = 1; w < kDistilThreads / 32; ++w) v = fmaxf(v, smem[w]);
-  __syncthreads();
-  return v;
+// A teacher's row, by one warp: tokens (-1 where there is none) and shares q to shared memory.
+struct TeacherRow {
+  float best, mass;
+  bool some, wrong;  // wrong: a class that is none, or a score that is no number
+};
+__device__ __forceinline__ TeacherRow ReadTeacher(const Teacher &t, int64_t r, int32_t classes,
+                                                  int32_t lane, int32_t *token, float *share) {
+  TeacherRow row;
+  bool wrong = false;
+  float best = -INFINITY;
+  for (int32_t j = lane; j < t.entries; j += 32) {
+    const int64_t at = r * t.entries + j, c = IntAt(t.tokens, t.tokens_64, at);
+    float score = -INFINITY;
+    wrong |= c < -1 || c >= classes;
+    if (c >= 0 && c < classes) {
+      score = TeacherScore(t, at);
+      wrong |= !(score < INFINITY);
+    }
+    best = fmaxf(best, score);
+    token[j] = c >= 0 && c < classes ? (int32_t)c : -1;
+    share[j] = score;
+  }
+  row.wrong = __any_sync(0xffffffffu, wrong);
+  row.best = WarpMaxF(best);
+  row.some = row.best > -INFINITY || row.wrong;
+  row.mass = 0.0f;
+  return row;
 }
-__device__ __forceinline__ float DistilSum(float v, float *smem) {
-  v = TeamSum(v);
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0f;
-  for (int w = 0; w < kDistilThreads / 32; ++w) v += smem[w];
-  __syncthreads();
-  return v;
+// ... the scores there become shares.
+__device__ __forceinline__ void ShareOut(const Teacher &t, TeacherRow &row, float k, int32_t lane,
+                                         float *share) {
+  float mass = 0.0f;
+  for (int32_t j = lane; j < t.entries; j += 32) {
+    const float part = row.best > -INFINITY ? Exp2((share[j] - row.best) * k) : 0.0f;
+    mass += part;
+    share[j] = part;
+  }
+  row.mass = WarpSumF(mass);
+  const float by = row.best > -INFINITY ? 1.0f / row.mass : 0.0f;
+  for (int32_t j = lane; j < t.entries; j += 32) share[j] *= by;
 }
 
-// A block per row: the student's largest score and sum, the teacher's distribution, the loss, and
-// the gradient T * (p - q) * scale.  kBackward: the norm is known, the upstream multiplies, and no
-// loss is written.
-template <typename T, bool kBackward>
-__global__ void __launch_bounds__(kDistilThreads)
-Distil(Rows<T> rows, Teacher t, float4 *norm, float *row_loss, int32_t scaled_loss, T *grad,
-       int64_t outer_stride, int64_t inner_stride, const DistilScale *scale, k2b200_row_grad up,
-       int32_t unless_one) {
-  __shared__ float smem[kDistilThreads / 32];
-  __shared__ int32_t token[K2B200_MAX_TOP];
-  __shared__ float share[K2B200_MAX_TOP];
-  const int32_t r = blockIdx.x, tid = threadIdx.x, C = rows.classes;
-  if (kBackward && unless_one && up.grad[0] == 1.0f) return;
-  const RowPlace at = PlaceOf(rows, r);
-  T *out = grad ? grad + at.o * outer_stride + at.i * inner_stride : nullptr;
-  if (!at.counts) {
-    if (out)
-      for (int32_t c = tid; c < C; c += kDistilThreads) out[c] = FromFloat<T>(0.0f);
-    if (tid == 0 && row_loss) row_loss[r] = 0.0f;
-    return;
+// The teacher's classes among [begin, end) of a row, behind the stores of all others: a class that
+// comes several times has the sum of its shares, whoever writes it.
+template <typename T>
+__device__ __forceinline__ void WriteNamed(const Rows<T> &rows, const T *x, T *out, int32_t begin,
+                                           int32_t end, int32_t entries, const int32_t *token,
+                                           const float *share, int32_t tid, int32_t team,
+                                           float high, float k, float inverse, float by) {
+  for (int32_t j = tid; j < entries; j += team) {
+    const int32_t c = token[j];
+    if (c < begin || c >= end) continue;
+    float hit = 0.0f;
+    for (int32_t o = 0; o < entries; ++o) hit += token[o] == c ? share[o] : 0.0f;
+    out[c] = FromFloat<T>((Exp2((ToFloat(x[c]) - high) * k) * inverse - hit) * by);
   }
-  const T *x = rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride;
-  const float inverse_t = 1.0f / t.temperature, k = kLog2e / t.temperature;
-  // the teacher
-  bool bad = false, some = false;
-  float mine = -INFINITY;
-  int32_t my_token = -1;
-  if (tid < t.entries) {
-    const int64_t j = (int64_t)r * t.entries + tid, c = IntAt(t.tokens, t.tokens_64, j);
-    bad = c < -1 || c >= C;
-    if (c >= 0 && c < C) {
-      my_token = (int32_t)c;
-      mine = TeacherScore(t, j);
+}
+
+// Zeros for a row.
+template <typename T>
+__device__ __forceinline__ void WriteZeros(T *out, int32_t classes, int32_t first, int32_t last,
+                                           int32_t tid, int32_t team) {
+  const RowSpan<T> zeros(out, classes);
+  const float f[kPer<T>] = {};
+  for (int32_t j = first + tid; j < min(last, zeros.vectors); j += team)
+    Store(out, zeros, true, j, f);
+}
+
+template <int kTeam>
+struct DistilShared {
+  float high[kTeam / 32], sum[kTeam / 32];
+  float all_high, all_sum;  // of a block, for its cluster
+  int32_t some, wrong;
+};
+
+// kTeam threads per row and block with kVectors vectors each; kAgain: the row does not fit and is
+// read again for each pass.  Rows of a cluster of blocks (kTeam 256) are dealt out in slices.
+// loss: of the rows, or NULL and `partial` has the sum of each block's rows.
+template <typename T, int kTeam, int kVectors, bool kAgain>
+__global__ void __launch_bounds__(kTeam == 128 ? 128 : 256, MinBlocks(kTeam, kVectors))
+Distil(Rows<T> rows, Teacher t, float4 *norm, float *loss, double *partial, T *grad,
+       int64_t outer_stride, int64_t inner_stride, DistilBy by) {
+  extern __shared__ int32_t all_entries[];
+  __shared__ DistilShared<kTeam> all_shared[kTeam == 32 ? 8 : 1];
+  __shared__ float losses[kTeam == 32 ? 8 : 1];
+  LetNextStart();
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t tid = kTeam == 32 ? lane : (int32_t)threadIdx.x;
+  DistilShared<kTeam> &sh = all_shared[kTeam == 32 ? warp : 0];
+  int32_t *token = all_entries + (kTeam == 32 ? warp * 2 * t.entries : 0);
+  float *share = reinterpret_cast<float *>(token + t.entries);
+  const uint32_t cluster = kTeam == 256 ? ClusterSize() : 1,
+                 rank = kTeam == 256 ? ClusterRank() : 0;
+  const int32_t r = kTeam == 32 ? (int32_t)(blockIdx.x * (blockDim.x >> 5)) + warp
+                                : (int32_t)(blockIdx.x / cluster);
+  float row_loss = 0.0f;
+  if (r < rows.count) {
+    const RowPlace at = PlaceOf(rows, r);
+    T *out = grad ? grad + at.o * outer_stride + at.i * inner_stride : nullptr;
+    const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
+                          rows.classes);
+    const int32_t slice = (span.vectors + (int32_t)cluster - 1) / (int32_t)cluster;
+    const int32_t first = min(span.vectors, (int32_t)rank * slice),
+                  last = min(span.vectors, first + slice);
+    if (!at.counts) {
+      if (out)
+        WriteZeros(out, rows.classes, (int32_t)rank * slice,
+                   rank + 1 == cluster ? INT32_MAX : ((int32_t)rank + 1) * slice, tid, kTeam);
+    } else {
+      uint4 v[kVectors];
+      const auto each = [&](auto &&f) {
+        if constexpr (kAgain) {
+          for (int32_t tile = first; tile < last; tile += kTeam * kVectors) {
+            LoadTile<kTeam, kVectors>(v, span, tile, last, tid);
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i) f(Packed(v[i]), tile + i * kTeam + tid, i);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kVectors; ++i) f(Packed(v[i]), first + i * kTeam + tid, i);
+        }
+      };
+      if (!kAgain) LoadTile<kTeam, kVectors>(v, span, first, last, tid);
+      const float k = kLog2e / t.temperature;
+      TeacherRow teacher = {};
+      if (kTeam == 32 || warp == 0) {
+        teacher = ReadTeacher(t, r, rows.classes, lane, token, share);
+        if (kTeam > 32 && lane == 0) {
+          sh.some = teacher.some;
+          sh.wrong = teacher.wrong;
+        }
+      }
+      // the largest score
+      float high = -INFINITY;
+      each([&](uint4 &x, int32_t, int) { high = fmaxf(high, VectorMax(x, span.row)); });
+      high = WarpMaxF(high);
+      if (kTeam > 32) {
+        if (lane == 0) sh.high[warp] = high;
+        TeamSync<kTeam>();
+#pragma unroll
+        for (int w = 0; w < kTeam / 32; ++w) high = fmaxf(high, sh.high[w]);
+      }
+      float from = high == -INFINITY ? 0.0f : high;
+      // the sum, of two vectors at a time
+      float sums[2] = {0.0f, 0.0f};
+      each([&](uint4 &x, int32_t, int i) {
+        After(x, sums[i & 1]);
+        float f[kPer<T>];
+        Unpack(x, f, span.row);
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e) sums[i & 1] += Exp2((f[e] - from) * k);
+      });
+      float sum = WarpSumF(sums[0] + sums[1]);
+      if (kTeam == 32 || warp == 0) ShareOut(t, teacher, k, lane, share);
+      if (kTeam > 32) {
+        if (lane == 0) sh.sum[warp] = sum;
+        TeamSync<kTeam>();
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kTeam / 32; ++w) sum += sh.sum[w];
+        teacher.some = sh.some;
+        teacher.wrong = sh.wrong;
+      } else {
+        TeamSync<kTeam>();
+      }
+      if (kTeam == 256 && cluster > 1) {
+        if (tid == 0) {
+          sh.all_high = high;
+          sh.all_sum = sum;
+        }
+        ClusterSync();
+        for (uint32_t b = 0; b < cluster; ++b) high = fmaxf(high, ReadFrom(&sh.all_high, b));
+        from = high == -INFINITY ? 0.0f : high;
+        sum = 0.0f;
+        for (uint32_t b = 0; b < cluster; ++b) {
+          const float part = ReadFrom(&sh.all_sum, b);
+          if (part == 0.0f) continue;  // (nothing but -inf)
+          sum = fmaf(part, Exp2((ReadFrom(&sh.all_high, b) - from) * k), sum);
+        }
+        ClusterSync();  // nobody goes on while others read its memory
+      }
+      // the loss
+      if ((kTeam == 32 || warp == 0) && rank == 0) {
+        const float inverse_t = 1.0f / t.temperature, log_mass = logf(teacher.mass),
+                    log_sum = logf(sum);
+        float term = 0.0f;
+        for (int32_t j = lane; j < t.entries; j += 32) {
+          const float q = share[j];
+          if (token[j] < 0 || q == 0.0f) continue;
+          const float log_q =
+              (TeacherScore(t, (int64_t)r * t.entries + j) - teacher.best) * inverse_t - log_mass;
+          const float log_p = sum == 0.0f
+                                  ? -INFINITY
+                                  : (ToFloat(span.row[token[j]]) - from) * inverse_t - log_sum;
+          term += q * (log_q - log_p);
+        }
+        term = WarpSumF(term);
+        if (teacher.wrong || (teacher.some && sum != sum)) term = NAN;
+        row_loss = t.temperature * t.temperature * term;
+        if (norm && lane == 0) norm[r] = make_float4(from, sum, 0.0f, 0.0f);
+      }
+      if (out && !teacher.some) {
+        WriteZeros(out, rows.classes, (int32_t)rank * slice,
+                   rank + 1 == cluster ? INT32_MAX : ((int32_t)rank + 1) * slice, tid, kTeam);
+      } else if (out) {
+        if (by.device) WaitForPrevious();
+        const float times = t.temperature * (by.device ? by.device->rounded : by.host.rounded);
+        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
+        const float spread = teacher.wrong ? NAN : inverse * times;
+        each([&](uint4 &x, int32_t j, int) {
+          if (j >= last) return;
+          float f[kPer<T>];
+          Unpack(x, f, span.row);
+#pragma unroll
+          for (int e = 0; e < kPer<T>; ++e) f[e] = Exp2((f[e] - from) * k) * spread;
+          Store(out, span, aligned, j, f);
+        });
+        TeamSync<kTeam>();
+        if (!teacher.wrong)
+          WriteNamed(rows, span.row, out, max(0, span.Column(first)),
+                     min(span.classes, span.Column(last)), t.entries, token, share, tid, kTeam,
+                     from, k, inverse, times);
+      }
     }
+    if (loss && rank == 0 && tid == 0)
+      loss[r] = row_loss * by.host.rounded;
   }
-  const bool nan = __syncthreads_or(bad || mine != mine || mine == INFINITY);
-  const float best = DistilMax(mine, smem);
-  some = best > -INFINITY;
-  const float part = some && mine > -INFINITY ? Exp2((mine - best) * k) : 0.0f;
-  const float mass = DistilSum(part, smem);
-  const float q = nan ? NAN : some ? part / mass : 0.0f;
-  if (tid < t.entries) {
-    token[tid] = my_token;
-    share[tid] = my_token >= 0 ? q : 0.0f;
-  }
-  __syncthreads();
-  // the student
-  RowNorm n;
-  if (kBackward) {
-    const float4 v = norm[r];
-    n.high = v.x;
-    n.sum = v.y;
-  } else {
-    float high = -INFINITY;
-    for (int32_t c = tid; c < C; c += kDistilThreads) high = fmaxf(high, ToFloat(x[c]));
-    high = DistilMax(high, smem);
-    n.high = high == -INFINITY ? 0.0f : high;
-    float sum = 0.0f;
-    for (int32_t c = tid; c < C; c += kDistilThreads) sum += Exp2((ToFloat(x[c]) - n.high) * k);
-    n.sum = DistilSum(sum, smem);
-    float term = 0.0f;
-    if (my_token >= 0 && (q > 0.0f || q != q)) {
-      const float log_q = (mine - best) * inverse_t - logf(mass);
-      const float log_p = n.sum == 0.0f ? -INFINITY
-                                        : (ToFloat(x[my_token]) - n.high) * inverse_t - logf(n.sum);
-      term = q * (log_q - log_p);
+  if (loss) return;
+  // (the next kernel reads the scale too, and waits for nothing but this one's end)
+  if (by.device) WaitForPrevious();
+  if (kTeam == 32) {
+    if (lane == 0) losses[warp] = row_loss;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double sum = 0.0;
+      for (uint32_t w = 0; w < blockDim.x / 32; ++w) sum += losses[w];
+      partial[blockIdx.x] = sum;
     }
-    term = DistilSum(term, smem);
-    // a student row of NaN is NaN even where the teacher says nothing of it
-    if (nan || (some && n.sum != n.sum)) term = NAN;
-    if (tid == 0) {
-      const float loss = t.temperature * t.temperature * term;
-      row_loss[r] = scaled_loss ? loss * scale->rounded : loss;
-      if (norm) norm[r] = make_float4(n.high, n.sum, 0.0f, 0.0f);
-    }
-  }
-  if (!out) return;
-  const float by = t.temperature * scale->rounded *
-                   (kBackward ? up.grad[at.o * up.outer + at.i * up.inner] : 1.0f);
-  const float inverse = n.sum == 0.0f ? 0.0f : 1.0f / n.sum;
-  for (int32_t c = tid; c < C; c += kDistilThreads) {
-    float v = !some ? 0.0f : Exp2((ToFloat(x[c]) - n.high) * k) * inverse;
-    if (nan) v = NAN;
-    for (int32_t j = 0; j < t.entries; ++j)
-      if (token[j] == c) v -= share[j];
-    out[c] = FromFloat<T>(v * by);
+  } else if (rank == 0 && tid == 0) {
+    partial[blockIdx.x / cluster] = row_loss;
   }
 }
 
 __global__ void __launch_bounds__(1024)
-DistilLoss(const float *row_loss, int32_t rows, const DistilScale *scale, float *loss) {
+DistilLoss(const double *partial, int32_t parts, DistilBy by, float *loss) {
   __shared__ double smem[32];
+  WaitForPrevious();
   double sum = 0.0;
-  for (int32_t r = threadIdx.x; r < rows; r += 1024) sum += row_loss[r];
+  for (int32_t r = threadIdx.x; r < parts; r += 1024) sum += partial[r];
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int w = 0; w < 32; ++w) sum += smem[w];
-    *loss = (float)(sum * scale->exact);
+  if (threadIdx.x < 32) {
+    sum = smem[threadIdx.x];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (threadIdx.x == 0) *loss = (float)(sum * (by.device ? by.device->exact : by.host.exact));
+  }
+}
+
+// The gradient for an upstream, of rows whose norm is known: `items` parts of rows (kTeam 256) or
+// eight rows (kTeam 32), dealt out to the blocks there are.  unless_one: what is there stays where
+// the upstream is 1.
+template <typename T, int kTeam>
+__global__ void __launch_bounds__(256, 4)
+DistilBackward(Rows<T> rows, Teacher t, const float4 *norm, T *grad, int64_t outer_stride,
+               int64_t inner_stride, DistilBy by, k2b200_row_grad up, int32_t unless_one,
+               int64_t items, int32_t parts, int32_t part) {
+  constexpr int kTile = 4;
+  extern __shared__ int32_t all_entries[];
+  __shared__ int32_t flags[2];
+  if (unless_one && up.grad[0] == 1.0f) return;
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t tid = kTeam == 32 ? lane : (int32_t)threadIdx.x;
+  int32_t *token = all_entries + (kTeam == 32 ? warp * 2 * t.entries : 0);
+  float *share = reinterpret_cast<float *>(token + t.entries);
+  const float k = kLog2e / t.temperature;
+  const float scale = t.temperature * (by.device ? by.device->rounded : by.host.rounded);
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t r64 = kTeam == 32 ? item * (blockDim.x >> 5) + warp : item / parts;
+    if (r64 >= rows.count) continue;  // (a whole team)
+    const int32_t r = (int32_t)r64;
+    const int32_t first = kTeam == 32 ? 0 : (int32_t)(item % parts) * part;
+    const RowPlace at = PlaceOf(rows, r);
+    T *out = grad + at.o * outer_stride + at.i * inner_stride;
+    const int32_t zeros_end = kTeam == 32 ? INT32_MAX : first + part;
+    if (!at.counts) {
+      WriteZeros(out, rows.classes, first, zeros_end, tid, kTeam);
+      continue;
+    }
+    const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
+                          rows.classes);
+    const int32_t last = kTeam == 32 ? span.vectors : min(span.vectors, first + part);
+    uint4 v[kTile];
+    LoadTile<kTeam, kTile>(v, span, first, last, tid);
+    TeacherRow teacher = {};
+    if (kTeam == 32 || warp == 0) {
+      teacher = ReadTeacher(t, r, rows.classes, lane, token, share);
+      ShareOut(t, teacher, k, lane, share);
+      if (kTeam > 32 && lane == 0) {
+        flags[0] = teacher.some;
+        flags[1] = teacher.wrong;
+      }
+    }
+    TeamSync<kTeam>();
+    if (kTeam > 32) {
+      teacher.some = flags[0];
+      teacher.wrong = flags[1];
+    }
+    if (!teacher.some) {
+      WriteZeros(out, rows.classes, first, zeros_end, tid, kTeam);
+      TeamSync<kTeam>();
+      continue;
+    }
+    const float4 n = norm[r];
+    const float times = scale * up.grad[at.o * up.outer + at.i * up.inner];
+    const float inverse = n.y == 0.0f ? 0.0f : 1.0f / n.y;
+    const float spread = teacher.wrong ? NAN : inverse * times;
+    const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
+    for (int32_t tile = first; tile < last; tile += kTeam * kTile) {
+      if (tile != first) LoadTile<kTeam, kTile>(v, span, tile, last, tid);
+#pragma unroll
+      for (int i = 0; i < kTile; ++i) {
+        const int32_t j = tile + i * kTeam + tid;
+        if (j >= last) continue;
+        float f[kPer<T>];
+        Unpack(Packed(v[i]), f, span.row);
+#pragma unroll
+        for (int e = 0; e < kPer<T>; ++e) f[e] = Exp2((f[e] - n.x) * k) * spread;
+        Store(out, span, aligned, j, f);
+      }
+    }
+    TeamSync<kTeam>();
+    if (!teacher.wrong)
+      WriteNamed(rows, span.row, out, max(0, span.Column(first)),
+                 min(span.classes, span.Column(last)), t.entries, token, share, tid, kTeam, n.x,
+                 k, inverse, times);
+    TeamSync<kTeam>();  // the next row's entries come to the same place
   }
 }
 
@@ -189,27 +417,61 @@ int32_t CheckTeacher(const k2b200_teacher *t, const k2b200_class_rows *rows) {
   return kOk;
 }
 
+// Whether the rows that count are known to the device alone.
+bool CountedThere(const k2b200_class_rows *rows, const k2b200_teacher *t) {
+  return t->reduction == 2 && rows->lengths != nullptr;
+}
+
+DistilBy ByOf(const k2b200_class_rows *rows, const k2b200_teacher *t, const void *workspace) {
+  DistilBy by = {};
+  if (CountedThere(rows, t)) {
+    by.device = static_cast<const DistilScale *>(workspace);
+    return by;
+  }
+  const int64_t n = t->reduction == 2 ? std::max<int64_t>(1, rows->outer * rows->inner) : 1;
+  by.host.exact = (double)t->weight / (double)n;
+  by.host.rounded = (float)by.host.exact;
+  return by;
+}
+
 template <typename T>
 int32_t LaunchDistil(const k2b200_class_rows *rows, const k2b200_teacher *t, float *loss,
                      float *norm, void *grad, int64_t outer_stride, int64_t inner_stride,
                      void *workspace, cudaStream_t s) {
-  const int32_t num = (int32_t)(rows->outer * rows->inner);
-  DistilScale *scale = static_cast<DistilScale *>(workspace);
-  float *row_loss = reinterpret_cast<float *>(static_cast<char *>(workspace) + kDistilHead);
+  const Rows<T> r = RowsOf<T>(rows);
   const Teacher teacher = {t->tokens, t->scores, t->tokens_64, t->type, t->entries,
                            t->temperature};
-  DistilScaleOf<<<1, 1024, 0, s>>>(rows->lengths, rows->lengths_64, rows->outer, rows->inner,
-                                   t->weight, t->reduction == 2, scale);
-  NoteLaunch();
-  if (num > 0) {
-    Distil<T, false><<<num, kDistilThreads, 0, s>>>(
-        RowsOf<T>(rows), teacher, reinterpret_cast<float4 *>(norm),
-        t->reduction == 0 ? loss : row_loss, t->reduction == 0, static_cast<T *>(grad),
-        outer_stride, inner_stride, scale, k2b200_row_grad{}, 0);
+  const DistilBy by = ByOf(rows, t, workspace);
+  double *partial = reinterpret_cast<double *>(static_cast<char *>(workspace) + kDistilHead);
+  const RowPlan p = PlanRows(r);
+  const int64_t groups = p.team == 32 ? CeilDiv(r.count, p.rows_per_block) : r.count;
+  if (by.device) {
+    DistilCount<<<1, 1024, 0, s>>>(rows->lengths, rows->lengths_64, rows->outer, rows->inner,
+                                   t->weight, static_cast<DistilScale *>(workspace));
+    NoteLaunch();
+  }
+  if (r.count > 0) {
+    auto kernel = p.team == 32    ? (p.vectors == 1   ? Distil<T, 32, 1, false>
+                                     : p.vectors == 2 ? Distil<T, 32, 2, false>
+                                     : p.vectors == 4 ? Distil<T, 32, 4, false>
+                                                      : Distil<T, 32, 8, false>)
+                  : p.team == 128 ? (p.vectors == 4 ? Distil<T, 128, 4, false>
+                                                    : Distil<T, 128, 8, false>)
+                  : p.again       ? Distil<T, 256, 16, true>
+                  : p.vectors == 4 ? Distil<T, 256, 4, false>
+                  : p.vectors == 8 ? Distil<T, 256, 8, false>
+                                   : Distil<T, 256, 16, false>;
+    const size_t smem = (sizeof(int32_t) + sizeof(float)) * t->entries *
+                        (p.team == 32 ? p.rows_per_block : 1);
+    K2B_CUDA_OK(LaunchRows(kernel, groups * p.cluster, p.block, smem, p.cluster,
+                           by.device != nullptr, s, r, teacher, reinterpret_cast<float4 *>(norm),
+                           t->reduction == 0 ? loss : nullptr, partial, static_cast<T *>(grad),
+                           outer_stride, inner_stride, by));
     NoteLaunch();
   }
   if (t->reduction != 0) {
-    DistilLoss<<<1, 1024, 0, s>>>(row_loss, num, scale, loss);
+    K2B_CUDA_OK(LaunchRows(DistilLoss, 1, 1024, 0, 1, r.count > 0, s, partial, (int32_t)groups,
+                           by, loss));
     NoteLaunch();
   }
   K2B_CUDA_OK(cudaGetLastError());
@@ -221,12 +483,23 @@ int32_t LaunchDistilBackward(const k2b200_class_rows *rows, const k2b200_teacher
                              const float *norm, const k2b200_row_grad *up, int32_t unless_one,
                              void *grad, int64_t outer_stride, int64_t inner_stride,
                              const void *workspace, cudaStream_t s) {
+  const Rows<T> r = RowsOf<T>(rows);
   const Teacher teacher = {t->tokens, t->scores, t->tokens_64, t->type, t->entries,
                            t->temperature};
-  Distil<T, true><<<(uint32_t)(rows->outer * rows->inner), kDistilThreads, 0, s>>>(
-      RowsOf<T>(rows), teacher, reinterpret_cast<float4 *>(const_cast<float *>(norm)), nullptr, 0,
-      static_cast<T *>(grad), outer_stride, inner_stride,
-      static_cast<const DistilScale *>(workspace), *up, unless_one);
+  const RowPlan p = PlanRows(r);
+  // vectors of a row, wherever it begins, in parts of a block's four per thread
+  const int32_t part = 1024, parts = CeilDiv((int64_t)r.classes + kPer<T> - 1, kPer<T>) + 1;
+  const int32_t row_parts = p.team == 32 ? 1 : CeilDiv(parts, part);
+  const int64_t items = p.team == 32 ? CeilDiv(r.count, p.rows_per_block)
+                                     : (int64_t)r.count * row_parts;
+  const int64_t blocks = std::min<int64_t>(items, 8 * (int64_t)NumSms());
+  auto kernel = p.team == 32 ? DistilBackward<T, 32> : DistilBackward<T, 256>;
+  const int32_t threads = p.team == 32 ? p.block : 256;
+  const size_t smem =
+      (sizeof(int32_t) + sizeof(float)) * t->entries * (p.team == 32 ? p.rows_per_block : 1);
+  kernel<<<(uint32_t)blocks, threads, smem, s>>>(
+      r, teacher, reinterpret_cast<const float4 *>(norm), static_cast<T *>(grad), outer_stride,
+      inner_stride, ByOf(rows, t, workspace), *up, unless_one, items, row_parts, part);
   NoteLaunch();
   K2B_CUDA_OK(cudaGetLastError());
   return kOk;
@@ -237,7 +510,7 @@ int32_t LaunchDistilBackward(const k2b200_class_rows *rows, const k2b200_teacher
 extern "C" {
 
 size_t k2b200_distillation_workspace_bytes(const k2b200_class_rows *rows) {
-  return rows ? kDistilHead + sizeof(float) * (size_t)(rows->outer * rows->inner) : 0;
+  return rows ? kDistilHead + sizeof(double) * (size_t)(rows->outer * rows->inner) : 0;
 }
 
 int32_t k2b200_distillation(const k2b200_class_rows *rows, const k2b200_teacher *teacher,

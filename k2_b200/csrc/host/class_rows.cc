@@ -93,8 +93,8 @@ RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengt
   RequireCuda(scores, "logits");
   Require(scores.dim() >= 1 && FloatType(scores) >= 0,
           "logits must be [..., classes] of float32, float16 or bfloat16");
-  Require(scores.size(-1) >= 1 && scores.size(-1) < ((int64_t)1 << 31),
-          "logits must have at least one class, and fewer than 2^31");
+  Require(scores.size(-1) >= 1 && scores.size(-1) <= ((int64_t)1 << 30),
+          "logits must have 1 to 2^30 classes");
   const int64_t lead = scores.dim() - 1;
   RowsOf r;
   r.scores = scores.detach();
@@ -123,9 +123,9 @@ RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengt
   r.rows.num_classes = (int32_t)scores.size(-1);
   r.rows.outer = SizeOf(scores, 0, r.split);
   r.rows.inner = SizeOf(scores, r.split, lead);
-  Require(r.rows.outer < ((int64_t)1 << 31) && r.rows.inner < ((int64_t)1 << 31) &&
-              r.rows.outer * r.rows.inner < ((int64_t)1 << 31),
-          "logits must have fewer than 2^31 rows");
+  Require(r.rows.outer < ((int64_t)1 << 28) && r.rows.inner < ((int64_t)1 << 28) &&
+              r.rows.outer * r.rows.inner < ((int64_t)1 << 28),
+          "logits must have fewer than 2^28 rows");
   r.rows.outer_stride = outer_stride;
   r.rows.inner_stride = inner_stride;
   if (lengths.has_value()) {

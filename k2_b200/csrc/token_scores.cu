@@ -1,105 +1,407 @@
 // Log-probs of given classes, entropies and top classes of rows of scores, and their gradient.
+//
+// TokenScores holds a row in registers (class_rows.cuh).  Sums: with d_c = (x_c - high) log2 e and
+// e_c = 2^d_c, log p_c = (x_c - high) - ln sum e, and the entropy is ln sum e - ln 2 (sum e d) /
+// sum e.  Top classes: the threads' largest scores are themselves scores of the row, so that the
+// k-th largest of them bounds the row's k-th largest from below, and few scores lie above it (of
+// n threads about n ln(n / (n - k))); those are collected in shared memory, and each one's place
+// is the number of larger ones.  Where more lie above it than there is room for - ties, or many
+// large scores in one thread - the bound is raised by bisection over (score, class), which no two
+// classes share.
 #include "class_rows.cuh"
+
+#include <type_traits>
 
 namespace k2b {
 
-constexpr int kTokenThreads = 128;
-
-template <typename V>
-__device__ __forceinline__ V BlockMax(V v, V *smem) {
-  v = TeamMax(v);
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = smem[0];
-  for (int w = 1; w < kTokenThreads / 32; ++w) v = smem[w] > v ? smem[w] : v;
-  __syncthreads();
-  return v;
-}
-__device__ __forceinline__ float BlockSum(float v, float *smem) {
-  v = TeamSum(v);
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0f;
-  for (int w = 0; w < kTokenThreads / 32; ++w) v += smem[w];
-  __syncthreads();
-  return v;
-}
-
 struct TokenOut {
   const void *tokens;
-  int32_t tokens_64, top_k;
+  int32_t tokens_64, top_k, room;  // room: keys per team
   float *log_probs, *entropy, *top_log_probs;
   int32_t *top_tokens;
   float4 *norm;
 };
 
-// log p of a score.
-__device__ __forceinline__ float LogProb(float x, RowNorm n) {
-  return n.sum == 0.0f ? -INFINITY : (x - n.high) - logf(n.sum);
+// Keys that a team has room for: what lies above the bound, with some to spare.
+static inline int32_t RoomFor(int32_t top_k) {
+  return top_k == 0 ? 0 : top_k <= 8 ? 32 : top_k <= 16 ? 64 : top_k <= 32 ? 96
+                                          : top_k <= 64 ? 160
+                                                        : 288;
 }
 
-// A block per row, which it reads once for the largest score, once for the sums and once for each
-// of its top classes.
+constexpr uint32_t kOrderOfNone = 0x007fffffu;  // OrderOf(-inf)
+
+// The largest bound found that at least k of a warp's kGroups values per lane reach, where there
+// are so many; -inf else.  By bisection, until no more than a quarter too many reach it.
+template <int kGroups>
+__device__ __forceinline__ uint32_t BoundOf(const uint32_t (&order)[kGroups], int32_t k) {
+  uint32_t least = order[0], most = order[0];
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) {
+    least = min(least, order[g]);
+    most = max(most, order[g]);
+  }
+  if (k > 32 * kGroups) return kOrderOfNone;
+  uint32_t low = __reduce_min_sync(0xffffffffu, least);
+  uint32_t high = __reduce_max_sync(0xffffffffu, most) + 1;  // (NaN is not among them)
+  while (high - low > 1) {
+    const uint32_t mid = low + (high - low) / 2;
+    int32_t reach = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) reach += __popc(__ballot_sync(0xffffffffu, order[g] >= mid));
+    if (reach >= k) {
+      low = mid;
+      if (reach <= k + (k >> 2)) break;
+    } else {
+      high = mid;
+    }
+  }
+  return low;
+}
+
+template <int kTeam>
+struct TokenShared {
+  float high[kTeam / 32];
+  float2 sums[kTeam / 32];
+  int32_t counted[kTeam / 32];
+  int32_t found;
+  uint32_t bound;
+  float group[kTeam == 32 ? 1 : 2 * kTeam];
+};
+
+// What the blocks of a cluster tell each other.
+struct TokenCluster {
+  float high, sum, slope;
+  int32_t top;                       // keys in `list`
+  uint64_t list[K2B200_MAX_TOP];     // this block's, largest first
+  uint64_t others[8 * K2B200_MAX_TOP];
+};
+
+// What does not count: log-probs and entropy 0, no classes.
+__device__ __forceinline__ void SkipRow(const TokenOut &out, int32_t r, int32_t tid,
+                                        int32_t team) {
+  if (tid == 0) {
+    if (out.log_probs) out.log_probs[r] = 0.0f;
+    if (out.entropy) out.entropy[r] = 0.0f;
+    if (out.norm) out.norm[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  for (int32_t k = tid; k < out.top_k; k += team) {
+    out.top_log_probs[(int64_t)r * out.top_k + k] = 0.0f;
+    out.top_tokens[(int64_t)r * out.top_k + k] = -1;
+  }
+}
+
+__device__ __forceinline__ void WriteTop(const TokenOut &out, int32_t r, int32_t place,
+                                         uint64_t key, float high, float sum, float log_sum) {
+  const int64_t at = (int64_t)r * out.top_k + place;
+  out.top_tokens[at] = (int32_t)~(uint32_t)key;
+  out.top_log_probs[at] =
+      sum == 0.0f ? -INFINITY : (ScoreOf((uint32_t)(key >> 32)) - high) - log_sum;
+}
+
+// The values that a row has one of.
 template <typename T>
-__global__ void __launch_bounds__(kTokenThreads)
+__device__ __forceinline__ void Finish(const TokenOut &out, const Rows<T> &rows, int32_t r,
+                                       bool mine, int64_t token, float score, float high,
+                                       float sum, float slope) {
+  if (!mine) return;
+  const float log_sum = logf(sum);
+  const float h = sum == 0.0f ? 0.0f : log_sum - slope * kLn2 / sum;
+  if (out.entropy) out.entropy[r] = h;
+  if (out.norm) out.norm[r] = make_float4(high, sum, h, 0.0f);
+  if (out.log_probs)
+    out.log_probs[r] = token == -1                          ? 0.0f
+                       : token < 0 || token >= rows.classes ? NAN
+                       : sum == 0.0f                        ? -INFINITY
+                                                            : (score - high) - log_sum;
+}
+
+// kTeam threads per row and block with kVectors vectors each; kAgain: the row does not fit and is
+// read again for each pass.  Rows of a cluster of blocks (kTeam 256) are dealt out in slices.
+template <typename T, int kTeam, int kVectors, bool kTop, bool kAgain>
+__global__ void
+__launch_bounds__(kTeam == 128 ? 128 : 256, MinBlocks(kTeam, kVectors))
 TokenScores(Rows<T> rows, TokenOut out) {
-  __shared__ float smem[kTokenThreads / 32];
-  __shared__ uint64_t smem_key[kTokenThreads / 32];
-  const int32_t r = blockIdx.x, tid = threadIdx.x, C = rows.classes;
+  extern __shared__ uint64_t all_keys[];
+  __shared__ TokenShared<kTeam> all_shared[kTeam == 32 ? 8 : 1];
+  // (the smallest where blocks share no row)
+  __shared__ typename std::conditional<kTeam == 256, TokenCluster, int32_t>::type together;
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t tid = kTeam == 32 ? lane : (int32_t)threadIdx.x;
+  TokenShared<kTeam> &sh = all_shared[kTeam == 32 ? warp : 0];
+  uint64_t *keys = all_keys + (kTeam == 32 ? warp * out.room : 0);
+  const uint32_t cluster = kTeam == 256 ? ClusterSize() : 1,
+                 rank = kTeam == 256 ? ClusterRank() : 0;
+  const int32_t r = kTeam == 32 ? (int32_t)(blockIdx.x * (blockDim.x >> 5)) + warp
+                                : (int32_t)(blockIdx.x / cluster);
+  if (r >= rows.count) return;  // a whole team
   const RowPlace at = PlaceOf(rows, r);
   if (!at.counts) {
-    if (tid == 0) {
-      if (out.log_probs) out.log_probs[r] = 0.0f;
-      if (out.entropy) out.entropy[r] = 0.0f;
-      if (out.norm) out.norm[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    for (int32_t k = tid; k < out.top_k; k += kTokenThreads) {
-      out.top_log_probs[(int64_t)r * out.top_k + k] = 0.0f;
-      out.top_tokens[(int64_t)r * out.top_k + k] = -1;
-    }
-    return;
+    if (rank == 0) SkipRow(out, r, tid, kTeam);
+    return;  // (all blocks of the cluster)
   }
-  const T *x = rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride;
-  RowNorm n;
-  float high = -INFINITY;
-  for (int32_t c = tid; c < C; c += kTokenThreads) high = fmaxf(high, ToFloat(x[c]));
-  high = BlockMax(high, smem);
-  n.high = high == -INFINITY ? 0.0f : high;
-  float sum = 0.0f, slope = 0.0f;
-  for (int32_t c = tid; c < C; c += kTokenThreads) {
-    const float d = (ToFloat(x[c]) - n.high) * kLog2e, e = Exp2(d);
-    sum += e;
-    slope += e * fmaxf(d, -1e30f);  // 0 and not 0 * -inf where p = 0
+  const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
+                        rows.classes);
+  const int32_t slice = (span.vectors + (int32_t)cluster - 1) / (int32_t)cluster;
+  const int32_t first = min(span.vectors, (int32_t)rank * slice),
+                last = min(span.vectors, first + slice);
+
+  uint4 v[kVectors];
+  const auto each = [&](auto &&f) {
+    if constexpr (kAgain) {
+      for (int32_t tile = first; tile < last; tile += kTeam * kVectors) {
+        LoadTile<kTeam, kVectors>(v, span, tile, last, tid);
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) f(Packed(v[i]), tile + i * kTeam + tid, i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) f(Packed(v[i]), first + i * kTeam + tid, i);
+    }
+  };
+  if (!kAgain) LoadTile<kTeam, kVectors>(v, span, first, last, tid);
+  // the given class's score is on its way meanwhile
+  int64_t token = -1;
+  float token_score = 0.0f;
+  if (out.log_probs && tid == 0 && rank == 0) {
+    token = IntAt(out.tokens, out.tokens_64, r);
+    if (token >= 0 && token < rows.classes) token_score = ToFloat(span.row[token]);
   }
-  n.sum = BlockSum(sum, smem);
-  slope = BlockSum(slope, smem);
-  const float h = n.sum == 0.0f ? 0.0f : logf(n.sum) - slope * kLn2 / n.sum;
-  if (tid == 0) {
-    if (out.entropy) out.entropy[r] = h;
-    if (out.norm) out.norm[r] = make_float4(n.high, n.sum, h, 0.0f);
-    if (out.log_probs) {
-      const int64_t token = IntAt(out.tokens, out.tokens_64, r);
-      out.log_probs[r] = token == -1              ? 0.0f
-                         : token < 0 || token >= C ? NAN
-                                                   : LogProb(ToFloat(x[token]), n);
+
+  // the largest score, of the team and of two groups per thread
+  float group[2] = {-INFINITY, -INFINITY};
+  each([&](uint4 &x, int32_t, int i) {
+    float &g = group[2 * i / kVectors];
+    g = fmaxf(g, VectorMax(x, span.row));
+  });
+  float high = WarpMaxF(fmaxf(group[0], group[1]));
+  if (kTeam > 32) {
+    if (lane == 0) sh.high[warp] = high;
+    if (kTop) {
+      sh.group[tid] = group[0];
+      sh.group[kTeam + tid] = group[1];
+    }
+    TeamSync<kTeam>();
+#pragma unroll
+    for (int w = 0; w < kTeam / 32; ++w) high = fmaxf(high, sh.high[w]);
+  }
+  const float from = high == -INFINITY ? 0.0f : high;
+
+  // the sums, of two vectors at a time
+  float sums[2] = {0.0f, 0.0f}, slopes[2] = {0.0f, 0.0f};
+  if (out.entropy || out.norm) {
+    each([&](uint4 &x, int32_t, int i) {
+      After(x, sums[i & 1]);
+      float f[kPer<T>];
+      Unpack(x, f, span.row);
+#pragma unroll
+      for (int k = 0; k < kPer<T>; ++k) {
+        const float d = (f[k] - from) * kLog2e, e = Exp2(d);
+        sums[i & 1] += e;
+        slopes[i & 1] = fmaf(e, fmaxf(d, -1e30f), slopes[i & 1]);  // 0 and not 0 * -inf
+      }
+    });
+  } else {
+    each([&](uint4 &x, int32_t, int i) {
+      After(x, sums[i & 1]);
+      float f[kPer<T>];
+      Unpack(x, f, span.row);
+#pragma unroll
+      for (int k = 0; k < kPer<T>; ++k) sums[i & 1] += Exp2((f[k] - from) * kLog2e);
+    });
+  }
+  float sum = sums[0] + sums[1], slope = slopes[0] + slopes[1];
+  float2 both = WarpSum2F(sum, slope);
+  // the bound of the top classes, by the first warp while the others add up
+  const int32_t top_k = max(0, min(out.top_k, min(span.classes, span.Column(last)) -
+                                                 max(0, span.Column(first))));
+  if (kTop && (kTeam == 32 || warp == 0)) {
+    uint32_t bound;
+    if (kTeam == 32) {
+      const uint32_t one[1] = {OrderOf(fmaxf(group[0], group[1]))};
+      const uint32_t two[2] = {OrderOf(group[0]), OrderOf(group[1])};
+      bound = top_k <= 16 ? BoundOf(one, top_k) : BoundOf(two, top_k);
+    } else {
+      constexpr int kAll = 2 * kTeam / 32;
+      uint32_t order[kAll];
+#pragma unroll
+      for (int g = 0; g < kAll; ++g) order[g] = OrderOf(sh.group[32 * g + lane]);
+      if (top_k <= 32) {
+        uint32_t two[2] = {0, 0};
+#pragma unroll
+        for (int g = 0; g < kAll; ++g) two[g & 1] = max(two[g & 1], order[g]);
+        const uint32_t one[1] = {max(two[0], two[1])};
+        bound = top_k <= 16 ? BoundOf(one, top_k) : BoundOf(two, top_k);
+      } else {
+        bound = BoundOf(order, top_k);
+      }
+    }
+    if (lane == 0) {
+      sh.bound = bound;
+      sh.found = 0;
     }
   }
-  uint64_t last = ~0ull;
-  for (int32_t k = 0; k < out.top_k; ++k) {
-    uint64_t best = 0;
-    for (int32_t c = tid; c < C; c += kTokenThreads) {
-      const uint64_t key = KeyOf(ToFloat(x[c]), c);
-      if (key < last && key > best) best = key;
+  if (kTeam > 32) {
+    if (lane == 0) sh.sums[warp] = both;
+    TeamSync<kTeam>();
+    both = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kTeam / 32; ++w) {
+      both.x += sh.sums[w].x;
+      both.y += sh.sums[w].y;
     }
-    last = BlockMax(best, smem_key);
-    if (tid == 0) {
-      const int32_t c = (int32_t)~(uint32_t)last;
-      out.top_tokens[(int64_t)r * out.top_k + k] = c;
-      out.top_log_probs[(int64_t)r * out.top_k + k] = LogProb(ToFloat(x[c]), n);
+  } else if (kTop) {
+    TeamSync<kTeam>();
+  }
+  sum = both.x;
+  slope = both.y;
+
+  int32_t found = 0;
+  if (kTop) {
+    const bool odd = sum != sum;  // NaN, which VectorMax passes over
+    uint64_t bound = (uint64_t)sh.bound << 32;
+    const auto collect = [&](const uint4 &x, int32_t j, float least) {
+      if (!odd && VectorMax(x, span.row) < least) return;
+      float f[kPer<T>];
+      Unpack(x, f, span.row);
+#pragma unroll
+      for (int k = 0; k < kPer<T>; ++k)
+        if (!(f[k] < least)) {
+          const int32_t c = span.Column(j) + k;
+          const uint64_t key = KeyOf(f[k], c);
+          if (key >= bound && c >= 0 && c < span.classes && j < last) {
+            const int32_t place = atomicAdd(&sh.found, 1);
+            if (place < out.room) keys[place] = key;
+          }
+        }
+    };
+    const float least = ScoreOf(sh.bound);
+    each([&](uint4 &x, int32_t j, int) { collect(x, j, least); });
+    TeamSync<kTeam>();
+    found = sh.found;
+    if (found > out.room) {
+      // ties, or large scores side by side: between a bound that too many reach and one that
+      // too few do.  (The row is read again, from a cache: it would not stay in registers.)
+      const auto reach = [&](uint64_t key) {
+        int32_t n = 0;
+        for (int32_t j = first + tid; j < last; j += kTeam) {
+          float f[kPer<T>];
+          Unpack(span.Vector(j), f, span.row);
+#pragma unroll
+          for (int k = 0; k < kPer<T>; ++k) {
+            const int32_t c = span.Column(j) + k;
+            n += KeyOf(f[k], c) >= key && c >= 0 && c < span.classes;
+          }
+        }
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (kTeam > 32) {
+          TeamSync<kTeam>();
+          if (lane == 0) sh.counted[warp] = n;
+          TeamSync<kTeam>();
+          n = 0;
+#pragma unroll
+          for (int w = 0; w < kTeam / 32; ++w) n += sh.counted[w];
+        }
+        return n;
+      };
+      uint64_t low = bound, far = ~0ull, mid = bound + (1ull << 32);
+      for (;;) {
+        const int32_t n = reach(mid);
+        if (n >= top_k && n <= out.room) break;
+        if (n < top_k) far = mid; else low = mid;
+        // between keys of one score there are the classes
+        if ((far - 1) >> 32 == low >> 32)
+          low = max((unsigned long long)low, (low | 0xffffffffull) - (uint64_t)span.classes);
+        mid = low + (far - low) / 2;
+      }
+      bound = mid;
+      TeamSync<kTeam>();
+      if (tid == 0) sh.found = 0;
+      TeamSync<kTeam>();
+      const float higher = ScoreOf((uint32_t)(bound >> 32));
+      for (int32_t j = first + tid; j < last; j += kTeam) collect(span.Vector(j), j, higher);
+      TeamSync<kTeam>();
+      found = sh.found;
+    }
+  }
+
+  if constexpr (kTeam == 256) {
+    if (cluster > 1) {
+      // the first block of a cluster has the row's sums; each finds the places of its own keys
+      if (kTop)
+        for (int32_t k = tid; k < found; k += kTeam) {
+          const uint64_t key = keys[k];
+          int32_t place = 0;
+          for (int32_t o = 0; o < found; ++o) place += keys[o] > key;
+          if (place < top_k) together.list[place] = key;
+        }
+      if (tid == 0) {
+        together.high = high;
+        together.sum = sum;
+        together.slope = slope;
+        together.top = kTop ? top_k : 0;
+      }
+      ClusterSync();
+      for (uint32_t b = 0; b < cluster; ++b) high = fmaxf(high, ReadFrom(&together.high, b));
+      const float all_from = high == -INFINITY ? 0.0f : high;
+      sum = slope = 0.0f;
+      for (uint32_t b = 0; b < cluster; ++b) {
+        const float part = ReadFrom(&together.sum, b), h = ReadFrom(&together.high, b);
+        if (part == 0.0f) continue;  // (nothing but -inf)
+        const float d = (h - all_from) * kLog2e, by = Exp2(d);
+        sum = fmaf(part, by, sum);
+        // (d is far below 0 where `by` is 0)
+        slope = fmaf(by, fmaf(part, fmaxf(d, -1e30f), ReadFrom(&together.slope, b)), slope);
+      }
+      Finish<T>(out, rows, r, tid == 0 && rank == 0, token, token_score, all_from, sum, slope);
+      if (kTop) {
+        const float log_sum = logf(sum);
+        int32_t others = 0;
+        for (uint32_t b = 0; b < cluster; ++b) {
+          if (b == rank) continue;
+          const int32_t n = ReadFrom(&together.top, b);
+          for (int32_t k = tid; k < n; k += kTeam)
+            together.others[others + k] = ReadFrom(&together.list[k], b);
+          others += n;
+        }
+        __syncthreads();
+        for (int32_t k = tid; k < top_k; k += kTeam) {
+          const uint64_t key = together.list[k];
+          int32_t place = k, begin = 0;
+          for (uint32_t b = 0; b < cluster; ++b) {
+            if (b == rank) continue;
+            // how many of a list that falls are larger
+            const int32_t n = ReadFrom(&together.top, b);
+            int32_t low = 0, far = n;
+            while (low < far) {
+              const int32_t mid = (low + far) / 2;
+              if (together.others[begin + mid] > key) low = mid + 1; else far = mid;
+            }
+            place += low;
+            begin += n;
+          }
+          if (place < out.top_k) WriteTop(out, r, place, key, all_from, sum, log_sum);
+        }
+      }
+      ClusterSync();  // nobody leaves while others read its memory
+      return;
+    }
+  }
+  Finish<T>(out, rows, r, tid == 0, token, token_score, from, sum, slope);
+  if (kTop) {
+    const float log_sum = logf(sum);
+    for (int32_t k = tid; k < found; k += kTeam) {
+      const uint64_t key = keys[k];
+      int32_t place = 0;
+      for (int32_t o = 0; o < found; ++o) place += keys[o] > key;
+      if (place < out.top_k) WriteTop(out, r, place, key, from, sum, log_sum);
     }
   }
 }
 
+// ---------------------------------------------------------------------------
+// gradient
+// ---------------------------------------------------------------------------
 struct TokenGrad {
   const void *tokens;
   int32_t tokens_64, top_k;
@@ -115,43 +417,93 @@ __device__ __forceinline__ float GradAt(const k2b200_row_grad &g, RowPlace at, i
 
 // dL/dx_c = -p_c (all + slope * (log p_c + h)), with `all` the upstream of every log-prob of the
 // row; what a class gets as a given or a top one is added where it is.
-__device__ __forceinline__ float SpreadGrad(float x, float4 n, float inverse, float log_sum,
-                                            float all, float slope) {
-  const float d = x - n.x, p = Exp2(d * kLog2e) * inverse;
-  return p == 0.0f ? 0.0f : -p * (all + slope * (d - log_sum + n.z));
-}
+struct Spread {
+  float high, inverse, all, slope, offset;
+  __device__ __forceinline__ float operator()(float x) const {
+    const float d = x - high, p = Exp2(d * kLog2e) * inverse;
+    return p == 0.0f ? 0.0f : -p * fmaf(slope, d + offset, all);
+  }
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kTokenThreads)
-TokenScoresBackward(Rows<T> rows, TokenGrad g, T *grad) {
-  __shared__ float top_grad[K2B200_MAX_TOP];
-  const int32_t r = blockIdx.x, tid = threadIdx.x, C = rows.classes;
+// A team per row and kTile vectors per thread of it at a time: the norm is known, so every class
+// is on its own.  The classes that are a given or a top one are written again behind the others.
+template <typename T, int kTeam, bool kTop>
+__global__ void __launch_bounds__(256, 4)
+TokenScoresBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t part) {
+  constexpr int kTile = 4;
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t tid = kTeam == 32 ? lane : (int32_t)threadIdx.x;
+  const int32_t r = kTeam == 32 ? (int32_t)(blockIdx.x * (blockDim.x >> 5)) + warp
+                                : (int32_t)(blockIdx.x / (uint32_t)parts);
+  if (r >= rows.count) return;
+  const int32_t slice = kTeam == 32 ? 0 : (int32_t)(blockIdx.x % (uint32_t)parts);
   const RowPlace at = PlaceOf(rows, r);
   T *out = grad + at.o * g.outer_stride + at.i * g.inner_stride;
   if (!at.counts) {
-    for (int32_t c = tid; c < C; c += kTokenThreads) out[c] = FromFloat<T>(0.0f);
+    const RowSpan<T> zeros(out, rows.classes);
+    const float f[kPer<T>] = {};
+    const int32_t end = kTeam == 32 ? zeros.vectors : min(zeros.vectors, (slice + 1) * part);
+    for (int32_t j = slice * part + tid; j < end; j += kTeam) Store(out, zeros, true, j, f);
     return;
   }
-  const T *x = rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride;
-  const int32_t *top = g.top_tokens + (int64_t)r * g.top_k;
-  for (int32_t k = tid; k < g.top_k; k += kTokenThreads) top_grad[k] = GradAt(g.top, at, k);
-  __syncthreads();
+  const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
+                        rows.classes);
+  const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
+  const int32_t first = slice * part,
+                last = kTeam == 32 ? span.vectors : min(span.vectors, first + part);
+  uint4 v[kTile];
+  LoadTile<kTeam, kTile>(v, span, first, last, tid);
   const float4 n = g.norm[r];
   const int64_t token = g.log_probs.grad ? IntAt(g.tokens, g.tokens_64, r) : -1;
-  const float token_grad = token == -1              ? 0.0f
-                           : token < 0 || token >= C ? NAN
-                                                     : GradAt(g.log_probs, at);
-  float all = token_grad;
-  for (int32_t k = 0; k < g.top_k; ++k) all += top_grad[k];
-  const float slope = GradAt(g.entropy, at);
-  const float inverse = n.y == 0.0f ? 0.0f : 1.0f / n.y, log_sum = logf(n.y);
-  for (int32_t c = tid; c < C; c += kTokenThreads) {
-    float v = SpreadGrad(ToFloat(x[c]), n, inverse, log_sum, all, slope);
-    if (c == token) v += token_grad;
-    for (int32_t k = 0; k < g.top_k; ++k)
-      if (c == top[k]) v += top_grad[k];
-    out[c] = FromFloat<T>(v);
+  const bool some = token >= 0 && token < rows.classes;
+  const float token_grad = token == -1 ? 0.0f : some ? GradAt(g.log_probs, at) : NAN;
+  float top_sum = 0.0f;
+  if (kTop) {
+    // (each warp for itself)
+    for (int32_t k = lane; k < g.top_k; k += 32) top_sum += GradAt(g.top, at, k);
+    top_sum = WarpSumF(top_sum);
   }
+  Spread spread;
+  spread.high = n.x;
+  spread.inverse = n.y == 0.0f ? 0.0f : 1.0f / n.y;
+  spread.all = token_grad + top_sum;
+  spread.slope = GradAt(g.entropy, at);
+  spread.offset = n.z - logf(n.y);
+  for (int32_t tile = first; tile < last; tile += kTeam * kTile) {
+    if (tile != first) LoadTile<kTeam, kTile>(v, span, tile, last, tid);
+#pragma unroll
+    for (int i = 0; i < kTile; ++i) {
+      const int32_t j = tile + i * kTeam + tid;
+      if (j >= last) continue;
+      float f[kPer<T>];
+      Unpack(Packed(v[i]), f, span.row);
+#pragma unroll
+      for (int k = 0; k < kPer<T>; ++k) f[k] = spread(f[k]);
+      Store(out, span, aligned, j, f);
+    }
+  }
+  // behind the stores of the other threads: the token, unless a top class, and the top classes
+  TeamSync<kTeam>();
+  const int32_t begin = max(0, span.Column(first)),
+                end = min(span.classes, span.Column(last));
+  const auto mine = [&](int64_t c) { return c >= begin && c < end; };
+  bool token_is_top = false;
+  if (kTop) {
+    const int32_t *top = g.top_tokens + (int64_t)r * g.top_k;
+    for (int32_t k = tid; k < g.top_k; k += kTeam) {
+      const int32_t c = top[k];
+      if (!mine(c)) continue;
+      float value = spread(ToFloat(span.row[c])) + GradAt(g.top, at, k);
+      if (c == token) value += token_grad;
+      out[c] = FromFloat<T>(value);
+    }
+    if (some && tid < 32) {
+      for (int32_t k = lane; k < g.top_k; k += 32) token_is_top |= top[k] == token;
+      token_is_top = __any_sync(0xffffffffu, token_is_top);
+    }
+  }
+  if (tid == 0 && some && !token_is_top && mine(token))
+    out[token] = FromFloat<T>(spread(ToFloat(span.row[token])) + token_grad);
 }
 
 }  // namespace k2b
@@ -160,20 +512,49 @@ using namespace k2b;
 
 namespace {
 
-template <typename T>
+template <typename T, bool kTop>
 int32_t LaunchTokenScores(const k2b200_class_rows *rows, const TokenOut &out, cudaStream_t s) {
-  TokenScores<T><<<(uint32_t)(rows->outer * rows->inner), kTokenThreads, 0, s>>>(RowsOf<T>(rows),
-                                                                                 out);
+  const Rows<T> r = RowsOf<T>(rows);
+  const RowPlan p = PlanRows(r);
+  const int64_t blocks = p.team == 32 ? CeilDiv(r.count, p.rows_per_block)
+                                      : (int64_t)r.count * p.cluster;
+  const size_t smem = sizeof(uint64_t) * out.room * (p.team == 32 ? p.rows_per_block : 1);
+  void (*kernel)(Rows<T>, TokenOut) =
+      p.team == 32    ? (p.vectors == 1   ? TokenScores<T, 32, 1, kTop, false>
+                         : p.vectors == 2 ? TokenScores<T, 32, 2, kTop, false>
+                         : p.vectors == 4 ? TokenScores<T, 32, 4, kTop, false>
+                                          : TokenScores<T, 32, 8, kTop, false>)
+      : p.team == 128 ? (p.vectors == 4 ? TokenScores<T, 128, 4, kTop, false>
+                                        : TokenScores<T, 128, 8, kTop, false>)
+      : p.again       ? TokenScores<T, 256, 16, kTop, true>
+      : p.vectors == 4 ? TokenScores<T, 256, 4, kTop, false>
+      : p.vectors == 8 ? TokenScores<T, 256, 8, kTop, false>
+                       : TokenScores<T, 256, 16, kTop, false>;
+  K2B_CUDA_OK(LaunchRows(kernel, blocks, p.block, smem, p.cluster, false, s, r, out));
   NoteLaunch();
-  K2B_CUDA_OK(cudaGetLastError());
   return kOk;
 }
 
 template <typename T>
 int32_t LaunchTokenBackward(const k2b200_class_rows *rows, const TokenGrad &g, void *grad,
                             cudaStream_t s) {
-  TokenScoresBackward<T><<<(uint32_t)(rows->outer * rows->inner), kTokenThreads, 0, s>>>(
-      RowsOf<T>(rows), g, static_cast<T *>(grad));
+  const Rows<T> r = RowsOf<T>(rows);
+  const RowPlan p = PlanRows(r);
+  T *out = static_cast<T *>(grad);
+  const bool top = g.top_k > 0;
+  // vectors of a row, wherever it begins, in parts of 1024: a block's four per thread
+  const int32_t vectors =
+      (int32_t)((rows->num_classes + kPer<T> - 1) / kPer<T>) + (kPer<T> > 1 ? 1 : 0);
+  if (p.team == 32) {
+    auto kernel = top ? TokenScoresBackward<T, 32, true> : TokenScoresBackward<T, 32, false>;
+    kernel<<<CeilDiv(r.count, p.rows_per_block), p.block, 0, s>>>(r, g, out, 1, 0);
+  } else {
+    const int32_t part = 1024, parts = CeilDiv(vectors, part);
+    K2B_REQUIRE((int64_t)parts * r.count < ((int64_t)1 << 31), "too many rows of %d classes",
+                rows->num_classes);
+    auto kernel = top ? TokenScoresBackward<T, 256, true> : TokenScoresBackward<T, 256, false>;
+    kernel<<<(uint32_t)((int64_t)parts * r.count), 256, 0, s>>>(r, g, out, parts, part);
+  }
   NoteLaunch();
   K2B_CUDA_OK(cudaGetLastError());
   return kOk;
@@ -196,11 +577,18 @@ int32_t k2b200_token_scores(const k2b200_class_rows *rows, const void *tokens, i
               "tokens and log_probs are given together");
   K2B_REQUIRE(top_k == 0 || (top_log_probs && top_tokens), "NULL pointer");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const TokenOut out = {tokens,        tokens_64,  top_k, log_probs, entropy,
-                        top_log_probs, top_tokens, reinterpret_cast<float4 *>(norm)};
-  return rows->type == K2B200_F32   ? LaunchTokenScores<float>(rows, out, s)
-         : rows->type == K2B200_F16 ? LaunchTokenScores<__half>(rows, out, s)
-                                    : LaunchTokenScores<__nv_bfloat16>(rows, out, s);
+  const TokenOut out = {tokens,     tokens_64,     top_k,
+                        RoomFor(top_k), log_probs, entropy,
+                        top_log_probs,  top_tokens, reinterpret_cast<float4 *>(norm)};
+  const bool top = top_k > 0;
+  auto launch =
+      rows->type == K2B200_F32   ? (top ? LaunchTokenScores<float, true>
+                                        : LaunchTokenScores<float, false>)
+      : rows->type == K2B200_F16 ? (top ? LaunchTokenScores<__half, true>
+                                        : LaunchTokenScores<__half, false>)
+                                 : (top ? LaunchTokenScores<__nv_bfloat16, true>
+                                        : LaunchTokenScores<__nv_bfloat16, false>);
+  return launch(rows, out, s);
 }
 
 int32_t k2b200_token_scores_backward(const k2b200_class_rows *rows, const void *tokens,
