@@ -30,8 +30,9 @@ template <typename T>
 struct Rows {
   const T *scores;
   int32_t classes, count;
-  uint32_t inner;
+  uint32_t inner, inverse, shift;  // r / inner = r * inverse >> shift for r < 2^28
   int64_t outer_stride, inner_stride;
+  const T *begin, *end;  // the first class of all rows, and behind the last one
   const void *lengths;
   int32_t lengths_64;
 };
@@ -50,7 +51,7 @@ __device__ __forceinline__ int64_t IntAt(const void *ints, int32_t is_64, int64_
 template <typename T>
 __device__ __forceinline__ RowPlace PlaceOf(const Rows<T> &rows, int32_t r) {
   RowPlace p;
-  const uint32_t o = (uint32_t)r / rows.inner;
+  const uint32_t o = (uint32_t)((uint64_t)(uint32_t)r * rows.inverse >> rows.shift);
   p.o = o;
   p.i = (uint32_t)r - o * rows.inner;
   p.counts = rows.lengths == nullptr || p.i < IntAt(rows.lengths, rows.lengths_64, p.o);
@@ -81,6 +82,38 @@ __device__ __forceinline__ float Exp2(float x) {
   return y;
 }
 
+// Two numbers in one instruction each, rounded as by single ones.
+struct Two {
+  uint64_t bits;
+};
+__device__ __forceinline__ Two MakeTwo(float a, float b) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.bits) : "f"(a), "f"(b));
+  return t;
+}
+__device__ __forceinline__ float2 Split(Two t) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(t.bits));
+  return f;
+}
+__device__ __forceinline__ Two Add(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two Mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two Fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r.bits)
+      : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+
 // Order of scores: an unsigned number that grows with the score, 0 for none.  NaN comes before all
 // numbers and -0 equals +0.  With the class below it, two keys of a row are never equal.
 __device__ __forceinline__ uint32_t OrderOf(float v) {
@@ -101,27 +134,51 @@ __device__ __forceinline__ uint64_t KeyOf(float v, int32_t c) {
 template <typename T>
 constexpr int kPer = 16 / (int)sizeof(T);
 
-__device__ __forceinline__ void Unpack(uint4 v, float (&f)[4], const float *) {
-  f[0] = __uint_as_float(v.x);
-  f[1] = __uint_as_float(v.y);
-  f[2] = __uint_as_float(v.z);
-  f[3] = __uint_as_float(v.w);
+// Scores 2k and 2k + 1 of a vector.
+template <int kPair>
+__device__ __forceinline__ float2 PairOf(const uint4 &v, const float *) {
+  return kPair == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
+                    : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
 }
-__device__ __forceinline__ void Unpack(uint4 v, float (&f)[8], const __nv_bfloat16 *) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    f[2 * k] = __uint_as_float(w[k] << 16);
-    f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+template <int kPair>
+__device__ __forceinline__ uint32_t WordOf(const uint4 &v) {
+  return kPair == 0 ? v.x : kPair == 1 ? v.y : kPair == 2 ? v.z : v.w;
+}
+template <int kPair>
+__device__ __forceinline__ float2 PairOf(const uint4 &v, const __nv_bfloat16 *) {
+  const uint32_t w = WordOf<kPair>(v);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <int kPair>
+__device__ __forceinline__ float2 PairOf(const uint4 &v, const __half *) {
+  const uint32_t w = WordOf<kPair>(v);
+  __half2 h;
+  memcpy(&h, &w, 4);
+  return __half22float2(h);
+}
+template <typename T>
+__device__ __forceinline__ void Unpack(const uint4 &v, float (&f)[kPer<T>], const T *type) {
+  const float2 a = PairOf<0>(v, type), b = PairOf<1>(v, type);
+  f[0] = a.x;
+  f[1] = a.y;
+  f[2] = b.x;
+  f[3] = b.y;
+  if constexpr (kPer<T> == 8) {
+    const float2 c = PairOf<2>(v, type), d = PairOf<3>(v, type);
+    f[4] = c.x;
+    f[5] = c.y;
+    f[6] = d.x;
+    f[7] = d.y;
   }
 }
-__device__ __forceinline__ void Unpack(uint4 v, float (&f)[8], const __half *) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-    f[2 * k] = p.x;
-    f[2 * k + 1] = p.y;
+// f(pair, index) for the pairs of a vector.
+template <typename T, typename F>
+__device__ __forceinline__ void EachPair(const uint4 &v, const T *type, F &&f) {
+  f(PairOf<0>(v, type), 0);
+  f(PairOf<1>(v, type), 1);
+  if constexpr (kPer<T> == 8) {
+    f(PairOf<2>(v, type), 2);
+    f(PairOf<3>(v, type), 3);
   }
 }
 __device__ __forceinline__ uint4 Pack(const float (&f)[4], const float *) {
@@ -153,8 +210,8 @@ __device__ __forceinline__ uint4 &Packed(uint4 &v) {
 }
 // ... and does not unpack it before `sum` is what it is here: it would unpack all of a row's vectors
 // at once otherwise.
-__device__ __forceinline__ void After(uint4 &v, float &sum) {
-  asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w), "+f"(sum));
+__device__ __forceinline__ void After(uint4 &v, Two &sum) {
+  asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w), "+l"(sum.bits));
 }
 
 // The largest of a vector's scores; NaN are passed over.
@@ -223,37 +280,88 @@ struct RowSpan {
   }
 };
 
-// Vectors tile + i * kTeam + tid for i < kVectors of those before `last`.
+// Elements [begin, end) of a vector, -inf elsewhere.
+__device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end, const float *t) {
+  const uint4 low = LowestVector(t);
+  return make_uint4(begin <= 0 && end > 0 ? v.x : low.x, begin <= 1 && end > 1 ? v.y : low.y,
+                    begin <= 2 && end > 2 ? v.z : low.z, begin <= 3 && end > 3 ? v.w : low.w);
+}
+template <typename T>
+__device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end, const T *t) {
+  // (a shift by 32 or more leaves nothing)
+  const auto word = [&](uint32_t w, int32_t k, uint32_t low) {
+    uint32_t from, to;
+    asm("shl.b32 %0, %1, %2;" : "=r"(from) : "r"(~0u), "r"(max(0, 16 * begin - 32 * k)));
+    asm("shl.b32 %0, %1, %2;" : "=r"(to) : "r"(~0u), "r"(max(0, 16 * end - 32 * k)));
+    const uint32_t keep = from & ~to;
+    return (w & keep) | (low & ~keep);
+  };
+  const uint32_t low = LowestVector(t).x;
+  return make_uint4(word(v.x, 0, low), word(v.y, 1, low), word(v.z, 2, low), word(v.w, 3, low));
+}
+
+// Vectors tile + i * kTeam + tid for i < kVectors of those before `last`.  A vector that the row
+// shares with others is read as a whole where all of it lies between the first and the last class
+// of all rows, and element by element elsewhere.
 template <int kTeam, int kVectors, typename T>
 __device__ __forceinline__ void LoadTile(uint4 (&v)[kVectors], const RowSpan<T> &span,
-                                         int32_t tile, int32_t last, int32_t tid) {
+                                         const Rows<T> &rows, int32_t tile, int32_t last,
+                                         int32_t tid) {
+  const int32_t end = span.vectors - 1, rest = span.classes - span.Column(end);
+  const uint4 *at = reinterpret_cast<const uint4 *>(span.row - span.shift);
+  const bool front = span.shift != 0 && tile == 0,
+             tail = rest < kPer<T> && end >= tile && end < min(last, tile + kTeam * kVectors);
+  if ((!front || reinterpret_cast<const T *>(at) >= rows.begin) &&
+      (!tail || reinterpret_cast<const T *>(at + span.vectors) <= rows.end)) {
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i) {
-    const int32_t j = tile + i * kTeam + tid, c0 = span.Column(j);
-    v[i] = j < last && span.Whole(c0) ? *reinterpret_cast<const uint4 *>(span.row + c0)
-                                      : LowestVector(span.row);
-  }
-  // the row's first and last vector: two threads of the team at most, in one step of a warp
-  // unless one thread has both
-  const int32_t end = span.vectors - 1;
-  int32_t edge = tile == 0 && tid == 0 && !span.Whole(span.Column(0)) ? 0 : -1;
-  int32_t more = end > 0 && end >= tile && end < min(last, tile + kTeam * kVectors) &&
-                         ((end - tile) & (kTeam - 1)) == tid && !span.Whole(span.Column(end))
-                     ? end
-                     : -1;
-  if (edge < 0) {
-    edge = more;
-    more = -1;
-  }
-  while (edge >= 0) {
-    const uint4 e = span.Edge(edge);
-    const int32_t slot = (edge - tile) / kTeam;
+    for (int i = 0; i < kVectors; ++i) {
+      const int32_t j = tile + i * kTeam + tid;
+      v[i] = j < last ? at[j] : LowestVector(span.row);
+    }
+    if (front && tid == 0) v[0] = Keep(v[0], span.shift, kPer<T>, span.row);
+    if (tail) {
+      const int32_t slot = (end - tile) / kTeam;
+      const bool mine = ((end - tile) & (kTeam - 1)) == tid;
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      if (i == slot) v[i] = e;
-    edge = more;
-    more = -1;
+      for (int i = 0; i < kVectors; ++i)
+        if (i == slot) {
+          const uint4 kept = Keep(v[i], 0, rest, span.row);
+          if (mine) v[i] = kept;
+        }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      const int32_t j = tile + i * kTeam + tid;
+      v[i] = j < last && span.Whole(span.Column(j)) ? at[j] : LowestVector(span.row);
+    }
+#pragma unroll 1
+    for (int32_t both = 0; both < 2; ++both) {
+      const int32_t j = both ? end : 0;
+      if (j < tile || j >= min(last, tile + kTeam * kVectors) ||
+          ((j - tile) & (kTeam - 1)) != tid || span.Whole(span.Column(j)))
+        continue;
+      const uint4 e = span.Edge(j);
+      const int32_t slot = (j - tile) / kTeam;
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i)
+        if (i == slot) v[i] = e;
+    }
   }
+}
+
+// Sums of 2^d and of d 2^d over a vector, d = (x - high) * k.
+template <bool kSlope, typename T>
+__device__ __forceinline__ void AddVector(const uint4 &v, const T *type, float high, float k,
+                                          Two &sum, Two &slope) {
+  const Two minus = MakeTwo(-high, -high), by = MakeTwo(k, k);
+  EachPair(v, type, [&](float2 x, int) {
+    const float2 d = Split(Mul(Add(MakeTwo(x.x, x.y), minus), by));
+    const Two e = MakeTwo(Exp2(d.x), Exp2(d.y));
+    sum = Add(sum, e);
+    // 0 and not 0 * -inf where p = 0
+    if (kSlope) slope = Fma(e, MakeTwo(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), slope);
+  });
 }
 
 // Values for the classes of vector j into another row of the same length; `aligned`: both rows
@@ -298,6 +406,14 @@ __device__ __forceinline__ float2 WarpSum2F(float a, float b) {
 // Blocks of an SM that a kernel is compiled for: the registers are the row's and some 40 more.
 constexpr int MinBlocks(int team, int vectors) {
   return (vectors >= 16 ? 2 : vectors >= 8 ? 3 : 4) * (team == 128 ? 2 : 1);
+}
+
+// Adds sums of 2^d and d 2^d whose d is by `by` * log2 e too high (-inf: there are none).
+__device__ __forceinline__ void Join(float &sum, float &slope, float more, float more_slope,
+                                     float by) {
+  const float d = by * kLog2e, e = Exp2(d);
+  sum = fmaf(more, e, sum);
+  slope = fmaf(e, fmaf(more, fmaxf(d, -1e30f), more_slope), slope);
 }
 
 template <int kTeam>
@@ -352,12 +468,12 @@ struct RowPlan {
   int32_t cluster;  // blocks per row
   bool again;       // the row does not fit and is read again
   int32_t block;    // threads of a block: `team`, or several warps that are a team each
-  int32_t rows_per_block;
+  int32_t rows_per_warp, rows_per_block;
 };
 
 template <typename T>
 static inline RowPlan PlanRows(const Rows<T> &r) {
-  RowPlan p = {32, 1, 1, false, 32, 1};
+  RowPlan p = {32, 1, 1, false, 32, 1, 1};
   const int64_t rows = r.count, size = sizeof(T);
   // its vectors: one more where it does not begin with one
   const bool whole = ((uintptr_t)r.scores | (uint64_t)(r.outer_stride * size) |
@@ -366,9 +482,10 @@ static inline RowPlan PlanRows(const Rows<T> &r) {
   const int32_t sms = NumSms();
   if (bytes <= 32 * 8 * 16) {
     while (bytes > 32 * 16 * p.vectors) p.vectors *= 2;
-    // few rows: a warp to an SM; many: eight rows to a block
-    p.rows_per_block = (int32_t)std::min<int64_t>(8, std::max<int64_t>(1, rows / sms));
-    p.block = 32 * p.rows_per_block;
+    // few rows: one to a warp, and warps to as many SMs as there are; many: four to a warp
+    p.rows_per_warp = rows >= 16 * 4 * (int64_t)sms ? 4 : 1;
+    p.block = 32 * (int32_t)std::min<int64_t>(4, std::max<int64_t>(1, rows / sms));
+    p.rows_per_block = p.block / 32 * p.rows_per_warp;
     return p;
   }
   p.team = p.block = bytes <= 128 * 8 * 16 ? 128 : 256;
@@ -435,7 +552,18 @@ static inline Rows<T> RowsOf(const k2b200_class_rows *rows) {
   r.scores = static_cast<const T *>(rows->scores);
   r.classes = rows->num_classes;
   r.count = (int32_t)(rows->outer * rows->inner);
-  r.inner = (uint32_t)rows->inner;
+  r.inner = (uint32_t)std::max<int64_t>(1, rows->inner);
+  // with 2^28 times the next power of two over it, r * the error of the quotient stays below 1
+  r.shift = 28;
+  while ((1u << (r.shift - 28)) < r.inner) ++r.shift;
+  r.inverse = (uint32_t)((((uint64_t)1 << r.shift) + r.inner - 1) / r.inner);
+  r.begin = r.end = r.scores;
+  for (int64_t o : {(int64_t)0, rows->outer - 1})
+    for (int64_t i : {(int64_t)0, rows->inner - 1}) {
+      const T *x = r.scores + o * rows->outer_stride + i * rows->inner_stride;
+      r.begin = std::min(r.begin, x);
+      r.end = std::max(r.end, x + r.classes);
+    }
   r.outer_stride = rows->outer_stride;
   r.inner_stride = rows->inner_stride;
   r.lengths = rows->lengths;

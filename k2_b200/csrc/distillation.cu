@@ -2,7 +2,7 @@
 // gradient.
 //
 // With q = softmax(t / T) over a row's entries and p = softmax(x / T) over its classes, the loss is
-// T^2 sum_j q_j (log q_j - log p_j) and its gradient T (p_c - sum_j q_j [c = j]).  Distil holds the
+// T^2 sum_j q_j (log q_j - log p_j) and its gradient T (p_c - sum_j q_j [c = j]).  Distil hold the
 // row in registers (class_rows.cuh), so that loss and gradient take one read and one write of it;
 // the gradient is for an upstream of 1, and DistilBackward makes it again for another one.  All
 // classes are written as if the teacher had named none, whole vectors at a time, and its classes
@@ -56,7 +56,8 @@ DistilCount(const void *lengths, int32_t lengths_64, int64_t outer, int64_t inne
   }
 }
 
-// A teacher's row, by one warp: tokens (-1 where there is none) and shares q to shared memory.
+// A teacher's row, by one warp, in two steps: tokens (-1 where there is none) and scores to shared
+// memory, then the scores' shares q in their place.
 struct TeacherRow {
   float best, mass;
   bool some, wrong;  // wrong: a class that is none, or a score that is no number
@@ -68,14 +69,12 @@ __device__ __forceinline__ TeacherRow ReadTeacher(const Teacher &t, int64_t r, i
   float best = -INFINITY;
   for (int32_t j = lane; j < t.entries; j += 32) {
     const int64_t at = r * t.entries + j, c = IntAt(t.tokens, t.tokens_64, at);
-    float score = -INFINITY;
-    wrong |= c < -1 || c >= classes;
-    if (c >= 0 && c < classes) {
-      score = TeacherScore(t, at);
-      wrong |= !(score < INFINITY);
-    }
+    float score = TeacherScore(t, at);
+    const bool there = c >= 0 && c < classes;
+    wrong |= c < -1 || c >= classes || (there && !(score < INFINITY));
+    if (!there) score = -INFINITY;
     best = fmaxf(best, score);
-    token[j] = c >= 0 && c < classes ? (int32_t)c : -1;
+    token[j] = there ? (int32_t)c : -1;
     share[j] = score;
   }
   row.wrong = __any_sync(0xffffffffu, wrong);
@@ -84,25 +83,40 @@ __device__ __forceinline__ TeacherRow ReadTeacher(const Teacher &t, int64_t r, i
   row.mass = 0.0f;
   return row;
 }
-// ... the scores there become shares.
-__device__ __forceinline__ void ShareOut(const Teacher &t, TeacherRow &row, float k, int32_t lane,
-                                         float *share) {
-  float mass = 0.0f;
+// k: log2 e / T.  Returns sum_j q_j ((t_j - best) - (x_j - high)), of which, over T, the loss is
+// made (RowLoss).
+template <typename T>
+__device__ __forceinline__ float ShareOut(const Teacher &t, TeacherRow &row, const T *x, float k,
+                                          float high, int32_t lane, const int32_t *token,
+                                          float *share) {
+  float mass = 0.0f, term = 0.0f;
   for (int32_t j = lane; j < t.entries; j += 32) {
-    const float part = row.best > -INFINITY ? Exp2((share[j] - row.best) * k) : 0.0f;
+    const float d = row.best > -INFINITY ? share[j] - row.best : -INFINITY, part = Exp2(d * k);
     mass += part;
+    if (part != 0.0f) term += part * (d - (ToFloat(x[token[j]]) - high));
     share[j] = part;
   }
-  row.mass = WarpSumF(mass);
+  const float2 both = WarpSum2F(mass, term);
+  row.mass = both.x;
   const float by = row.best > -INFINITY ? 1.0f / row.mass : 0.0f;
   for (int32_t j = lane; j < t.entries; j += 32) share[j] *= by;
+  return both.y * by;
+}
+// T^2 sum_j q_j (log q_j - log p_j), with log q_j = (t_j - best) / T - log mass and log p_j =
+// (x_j - high) / T - log sum.
+__device__ __forceinline__ float RowLoss(float temperature, const TeacherRow &row, float sum,
+                                         float term) {
+  if (row.wrong || (row.some && sum != sum)) return NAN;
+  if (!row.some) return 0.0f;
+  if (sum == 0.0f) return INFINITY;  // the student rules out every class
+  return temperature * fmaf(temperature, logf(sum) - logf(row.mass), term);
 }
 
 // The teacher's classes among [begin, end) of a row, behind the stores of all others: a class that
 // comes several times has the sum of its shares, whoever writes it.
 template <typename T>
-__device__ __forceinline__ void WriteNamed(const Rows<T> &rows, const T *x, T *out, int32_t begin,
-                                           int32_t end, int32_t entries, const int32_t *token,
+__device__ __forceinline__ void WriteNamed(const T *x, T *out, int32_t begin, int32_t end,
+                                           int32_t entries, const int32_t *token,
                                            const float *share, int32_t tid, int32_t team,
                                            float high, float k, float inverse, float by) {
   for (int32_t j = tid; j < entries; j += team) {
@@ -112,6 +126,36 @@ __device__ __forceinline__ void WriteNamed(const Rows<T> &rows, const T *x, T *o
     for (int32_t o = 0; o < entries; ++o) hit += token[o] == c ? share[o] : 0.0f;
     out[c] = FromFloat<T>((Exp2((ToFloat(x[c]) - high) * k) * inverse - hit) * by);
   }
+}
+// The same by one warp for up to 32 entries: most rows have no class twice, which one comparison of
+// all lanes finds out.
+template <typename T>
+__device__ __forceinline__ void WriteNamedFew(const T *x, T *out, int32_t entries,
+                                              const int32_t *token, const float *share,
+                                              int32_t lane, float high, float k, float inverse,
+                                              float by) {
+  const int32_t c = lane < entries ? token[lane] : -1;
+  const uint32_t same = __match_any_sync(0xffffffffu, c);
+  float hit = c >= 0 ? share[lane] : 0.0f;
+  if (__any_sync(0xffffffffu, c >= 0 && (same & (same - 1)) != 0)) {
+    hit = 0.0f;
+    for (int32_t o = 0; o < entries; ++o) hit += token[o] == c ? share[o] : 0.0f;
+  }
+  if (c >= 0)
+    out[c] = FromFloat<T>((Exp2((ToFloat(x[c]) - high) * k) * inverse - hit) * by);
+}
+
+// p_c * by for the classes of a vector, p_c = 2^((x_c - high) * k) / sum with 1 / sum in `by`.
+template <typename T>
+__device__ __forceinline__ void Spread(const uint4 &v, const T *type, float high, float k,
+                                       float by, float (&f)[kPer<T>]) {
+  const Two minus = MakeTwo(-high, -high), times = MakeTwo(k, k), scale = MakeTwo(by, by);
+  EachPair(v, type, [&](float2 x, int pair) {
+    const float2 d = Split(Mul(Add(MakeTwo(x.x, x.y), minus), times));
+    const float2 p = Split(Mul(MakeTwo(Exp2(d.x), Exp2(d.y)), scale));
+    f[2 * pair] = p.x;
+    f[2 * pair + 1] = p.y;
+  });
 }
 
 // Zeros for a row.
@@ -124,6 +168,111 @@ __device__ __forceinline__ void WriteZeros(T *out, int32_t classes, int32_t firs
     Store(out, zeros, true, j, f);
 }
 
+// Rows of up to 4 KB: a warp takes `per_warp` of them one after the other.  Lane q knows where the
+// q-th of them is and computes its loss.  loss: of the rows, or NULL and `partial` has the sum of
+// each block's rows.
+template <typename T, int kVectors>
+__global__ void __launch_bounds__(128, kVectors >= 8 ? 6 : 8)
+DistilWarps(Rows<T> rows, Teacher t, float4 *norm, float *loss, double *partial, T *grad,
+            int64_t outer_stride, int64_t inner_stride, DistilBy by, int32_t per_warp) {
+  extern __shared__ int32_t all_entries[];
+  __shared__ double losses[4];
+  LetNextStart();
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int32_t *token = all_entries + warp * 2 * t.entries;
+  float *share = reinterpret_cast<float *>(token + t.entries);
+  const int32_t first = (int32_t)(blockIdx.x * (blockDim.x >> 5) + warp) * per_warp,
+                mine = first + lane, taken = min(per_warp, rows.count - first);
+  const T *my_row = nullptr;
+  T *my_out = nullptr;
+  if (lane < taken) {
+    const RowPlace at = PlaceOf(rows, mine);
+    if (at.counts) my_row = rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride;
+    if (grad) my_out = grad + at.o * outer_stride + at.i * inner_stride;
+  }
+  const float k = kLog2e / t.temperature;
+  float my_high = 0.0f, my_sum = 0.0f, my_term = 0.0f;
+  TeacherRow my_teacher = {};
+  for (int32_t q = 0; q < taken; ++q) {
+    const T *row = reinterpret_cast<const T *>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(my_row), q));
+    T *out = reinterpret_cast<T *>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(my_out), q));
+    if (row == nullptr) {
+      if (out) WriteZeros(out, rows.classes, 0, INT32_MAX, lane, 32);
+      continue;
+    }
+    const RowSpan<T> span(row, rows.classes);
+    uint4 v[kVectors];
+    LoadTile<32, kVectors>(v, span, rows, 0, span.vectors, lane);
+    TeacherRow teacher = ReadTeacher(t, first + q, rows.classes, lane, token, share);
+    float high = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) high = fmaxf(high, VectorMax(Packed(v[i]), row));
+    high = WarpMaxF(high);
+    const float from = high == -INFINITY ? 0.0f : high;
+    Two sums[2] = {}, none;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      After(v[i], sums[i & 1]);
+      AddVector<false>(v[i], row, from, k, sums[i & 1], none);
+    }
+    const float2 s = Split(Add(sums[0], sums[1]));
+    const float sum = WarpSumF(s.x + s.y);
+    const float term = ShareOut(t, teacher, row, k, from, lane, token, share);
+    if (lane == q) {
+      my_high = from;
+      my_sum = sum;
+      my_term = term;
+      my_teacher = teacher;
+    }
+    if (out && !teacher.some) {
+      WriteZeros(out, rows.classes, 0, INT32_MAX, lane, 32);
+    } else if (out) {
+      if (by.device) WaitForPrevious();
+      const float times = t.temperature * (by.device ? by.device->rounded : by.host.rounded);
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float spread = teacher.wrong ? NAN : inverse * times;
+      const bool aligned = (((uintptr_t)out ^ (uintptr_t)row) & 15) == 0;
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) {
+        const int32_t j = i * 32 + lane;
+        if (j >= span.vectors) continue;
+        float f[kPer<T>];
+        Spread(Packed(v[i]), row, from, k, spread, f);
+        Store(out, span, aligned, j, f);
+      }
+      __syncwarp();
+      if (!teacher.wrong) {
+        if (t.entries <= 32)
+          WriteNamedFew(row, out, t.entries, token, share, lane, from, k, inverse, times);
+        else
+          WriteNamed(row, out, 0, rows.classes, t.entries, token, share, lane, 32, from, k,
+                     inverse, times);
+      }
+    }
+    __syncwarp();  // the next row's entries come to the same place
+  }
+  float row_loss = 0.0f;
+  if (lane < taken) {
+    if (my_row) row_loss = RowLoss(t.temperature, my_teacher, my_sum, my_term);
+    if (norm) norm[mine] = make_float4(my_high, my_sum, 0.0f, 0.0f);
+    if (loss) loss[mine] = row_loss * by.host.rounded;
+  }
+  if (loss) return;
+  // (the next kernel reads the scale too, and waits for nothing but this one's end)
+  if (by.device) WaitForPrevious();
+  double all = row_loss;
+  for (int32_t d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+  if (lane == 0) losses[warp] = all;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    all = 0.0;
+    for (uint32_t w = 0; w < blockDim.x / 32; ++w) all += losses[w];
+    partial[blockIdx.x] = all;
+  }
+}
+
 template <int kTeam>
 struct DistilShared {
   float high[kTeam / 32], sum[kTeam / 32];
@@ -131,173 +280,132 @@ struct DistilShared {
   int32_t some, wrong;
 };
 
-// kTeam threads per row and block with kVectors vectors each; kAgain: the row does not fit and is
+// A block of kTeam threads per row with kVectors vectors each; kAgain: the row does not fit and is
 // read again for each pass.  Rows of a cluster of blocks (kTeam 256) are dealt out in slices.
-// loss: of the rows, or NULL and `partial` has the sum of each block's rows.
 template <typename T, int kTeam, int kVectors, bool kAgain>
-__global__ void __launch_bounds__(kTeam == 128 ? 128 : 256, MinBlocks(kTeam, kVectors))
-Distil(Rows<T> rows, Teacher t, float4 *norm, float *loss, double *partial, T *grad,
-       int64_t outer_stride, int64_t inner_stride, DistilBy by) {
-  extern __shared__ int32_t all_entries[];
-  __shared__ DistilShared<kTeam> all_shared[kTeam == 32 ? 8 : 1];
-  __shared__ float losses[kTeam == 32 ? 8 : 1];
-  LetNextStart();
-  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int32_t tid = kTeam == 32 ? lane : (int32_t)threadIdx.x;
-  DistilShared<kTeam> &sh = all_shared[kTeam == 32 ? warp : 0];
-  int32_t *token = all_entries + (kTeam == 32 ? warp * 2 * t.entries : 0);
+__global__ void __launch_bounds__(kTeam, MinBlocks(kTeam, kVectors))
+DistilBlocks(Rows<T> rows, Teacher t, float4 *norm, float *loss, double *partial, T *grad,
+             int64_t outer_stride, int64_t inner_stride, DistilBy by) {
+  extern __shared__ int32_t token[];
+  __shared__ DistilShared<kTeam> sh;
   float *share = reinterpret_cast<float *>(token + t.entries);
+  LetNextStart();
+  const int32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t cluster = kTeam == 256 ? ClusterSize() : 1,
                  rank = kTeam == 256 ? ClusterRank() : 0;
-  const int32_t r = kTeam == 32 ? (int32_t)(blockIdx.x * (blockDim.x >> 5)) + warp
-                                : (int32_t)(blockIdx.x / cluster);
+  const int32_t r = (int32_t)(blockIdx.x / cluster);
+  const RowPlace at = PlaceOf(rows, r);
+  T *out = grad ? grad + at.o * outer_stride + at.i * inner_stride : nullptr;
+  const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
+                        rows.classes);
+  const int32_t slice = (span.vectors + (int32_t)cluster - 1) / (int32_t)cluster;
+  const int32_t first = min(span.vectors, (int32_t)rank * slice),
+                last = min(span.vectors, first + slice);
+  // (a row of the gradient may lie otherwise and have a vector more)
+  const int32_t zeros_first = (int32_t)rank * slice,
+                zeros_last = rank + 1 == cluster ? INT32_MAX : ((int32_t)rank + 1) * slice;
   float row_loss = 0.0f;
-  if (r < rows.count) {
-    const RowPlace at = PlaceOf(rows, r);
-    T *out = grad ? grad + at.o * outer_stride + at.i * inner_stride : nullptr;
-    const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
-                          rows.classes);
-    const int32_t slice = (span.vectors + (int32_t)cluster - 1) / (int32_t)cluster;
-    const int32_t first = min(span.vectors, (int32_t)rank * slice),
-                  last = min(span.vectors, first + slice);
-    if (!at.counts) {
-      if (out)
-        WriteZeros(out, rows.classes, (int32_t)rank * slice,
-                   rank + 1 == cluster ? INT32_MAX : ((int32_t)rank + 1) * slice, tid, kTeam);
-    } else {
-      uint4 v[kVectors];
-      const auto each = [&](auto &&f) {
-        if constexpr (kAgain) {
-          for (int32_t tile = first; tile < last; tile += kTeam * kVectors) {
-            LoadTile<kTeam, kVectors>(v, span, tile, last, tid);
+  if (!at.counts) {
+    if (out) WriteZeros(out, rows.classes, zeros_first, zeros_last, tid, kTeam);
+    if (norm && rank == 0 && tid == 0) norm[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  } else {
+    uint4 v[kVectors];
+    const auto each = [&](auto &&f) {
+      if constexpr (kAgain) {
+        for (int32_t tile = first; tile < last; tile += kTeam * kVectors) {
+          LoadTile<kTeam, kVectors>(v, span, rows, tile, last, tid);
 #pragma unroll
-            for (int i = 0; i < kVectors; ++i) f(Packed(v[i]), tile + i * kTeam + tid, i);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kVectors; ++i) f(Packed(v[i]), first + i * kTeam + tid, i);
+          for (int i = 0; i < kVectors; ++i) f(i, tile + i * kTeam + tid);
         }
-      };
-      if (!kAgain) LoadTile<kTeam, kVectors>(v, span, first, last, tid);
-      const float k = kLog2e / t.temperature;
-      TeacherRow teacher = {};
-      if (kTeam == 32 || warp == 0) {
-        teacher = ReadTeacher(t, r, rows.classes, lane, token, share);
-        if (kTeam > 32 && lane == 0) {
-          sh.some = teacher.some;
-          sh.wrong = teacher.wrong;
-        }
-      }
-      // the largest score
-      float high = -INFINITY;
-      each([&](uint4 &x, int32_t, int) { high = fmaxf(high, VectorMax(x, span.row)); });
-      high = WarpMaxF(high);
-      if (kTeam > 32) {
-        if (lane == 0) sh.high[warp] = high;
-        TeamSync<kTeam>();
-#pragma unroll
-        for (int w = 0; w < kTeam / 32; ++w) high = fmaxf(high, sh.high[w]);
-      }
-      float from = high == -INFINITY ? 0.0f : high;
-      // the sum, of two vectors at a time
-      float sums[2] = {0.0f, 0.0f};
-      each([&](uint4 &x, int32_t, int i) {
-        After(x, sums[i & 1]);
-        float f[kPer<T>];
-        Unpack(x, f, span.row);
-#pragma unroll
-        for (int e = 0; e < kPer<T>; ++e) sums[i & 1] += Exp2((f[e] - from) * k);
-      });
-      float sum = WarpSumF(sums[0] + sums[1]);
-      if (kTeam == 32 || warp == 0) ShareOut(t, teacher, k, lane, share);
-      if (kTeam > 32) {
-        if (lane == 0) sh.sum[warp] = sum;
-        TeamSync<kTeam>();
-        sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kTeam / 32; ++w) sum += sh.sum[w];
-        teacher.some = sh.some;
-        teacher.wrong = sh.wrong;
       } else {
-        TeamSync<kTeam>();
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) f(i, first + i * kTeam + tid);
       }
-      if (kTeam == 256 && cluster > 1) {
-        if (tid == 0) {
-          sh.all_high = high;
-          sh.all_sum = sum;
-        }
-        ClusterSync();
-        for (uint32_t b = 0; b < cluster; ++b) high = fmaxf(high, ReadFrom(&sh.all_high, b));
-        from = high == -INFINITY ? 0.0f : high;
-        sum = 0.0f;
-        for (uint32_t b = 0; b < cluster; ++b) {
-          const float part = ReadFrom(&sh.all_sum, b);
-          if (part == 0.0f) continue;  // (nothing but -inf)
-          sum = fmaf(part, Exp2((ReadFrom(&sh.all_high, b) - from) * k), sum);
-        }
-        ClusterSync();  // nobody goes on while others read its memory
+    };
+    if (!kAgain) LoadTile<kTeam, kVectors>(v, span, rows, first, last, tid);
+    const float k = kLog2e / t.temperature;
+    TeacherRow teacher = {};
+    if (warp == 0) {
+      teacher = ReadTeacher(t, r, rows.classes, lane, token, share);
+      if (lane == 0) {
+        sh.some = teacher.some;
+        sh.wrong = teacher.wrong;
       }
-      // the loss
-      if ((kTeam == 32 || warp == 0) && rank == 0) {
-        const float inverse_t = 1.0f / t.temperature, log_mass = logf(teacher.mass),
-                    log_sum = logf(sum);
-        float term = 0.0f;
-        for (int32_t j = lane; j < t.entries; j += 32) {
-          const float q = share[j];
-          if (token[j] < 0 || q == 0.0f) continue;
-          const float log_q =
-              (TeacherScore(t, (int64_t)r * t.entries + j) - teacher.best) * inverse_t - log_mass;
-          const float log_p = sum == 0.0f
-                                  ? -INFINITY
-                                  : (ToFloat(span.row[token[j]]) - from) * inverse_t - log_sum;
-          term += q * (log_q - log_p);
-        }
-        term = WarpSumF(term);
-        if (teacher.wrong || (teacher.some && sum != sum)) term = NAN;
-        row_loss = t.temperature * t.temperature * term;
+    }
+    // the largest score and the sum of each warp
+    float high = -INFINITY;
+    each([&](int i, int32_t) { high = fmaxf(high, VectorMax(Packed(v[i]), span.row)); });
+    high = WarpMaxF(high);
+    float from = high == -INFINITY ? 0.0f : high;
+    Two sums[2] = {}, none;
+    each([&](int i, int32_t) {
+      After(v[i], sums[i & 1]);
+      AddVector<false>(v[i], span.row, from, k, sums[i & 1], none);
+    });
+    const float2 s = Split(Add(sums[0], sums[1]));
+    const float warp_sum = WarpSumF(s.x + s.y);
+    if (lane == 0) {
+      sh.high[warp] = high;
+      sh.sum[warp] = warp_sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kTeam / 32; ++w) high = fmaxf(high, sh.high[w]);
+    from = high == -INFINITY ? 0.0f : high;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kTeam / 32; ++w)
+      sum = fmaf(sh.sum[w], Exp2((sh.high[w] - from) * k), sum);
+    teacher.some = sh.some;
+    teacher.wrong = sh.wrong;
+    if (kTeam == 256 && cluster > 1) {
+      if (tid == 0) {
+        sh.all_high = high;
+        sh.all_sum = sum;
+      }
+      ClusterSync();
+      for (uint32_t b = 0; b < cluster; ++b) high = fmaxf(high, ReadFrom(&sh.all_high, b));
+      from = high == -INFINITY ? 0.0f : high;
+      sum = 0.0f;
+      for (uint32_t b = 0; b < cluster; ++b)
+        sum = fmaf(ReadFrom(&sh.all_sum, b), Exp2((ReadFrom(&sh.all_high, b) - from) * k), sum);
+      ClusterSync();  // nobody goes on while others read its memory
+    }
+    if (warp == 0) {
+      const float term = ShareOut(t, teacher, span.row, k, from, lane, token, share);
+      if (rank == 0) {
+        row_loss = RowLoss(t.temperature, teacher, sum, term);
         if (norm && lane == 0) norm[r] = make_float4(from, sum, 0.0f, 0.0f);
       }
-      if (out && !teacher.some) {
-        WriteZeros(out, rows.classes, (int32_t)rank * slice,
-                   rank + 1 == cluster ? INT32_MAX : ((int32_t)rank + 1) * slice, tid, kTeam);
-      } else if (out) {
-        if (by.device) WaitForPrevious();
-        const float times = t.temperature * (by.device ? by.device->rounded : by.host.rounded);
-        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
-        const float spread = teacher.wrong ? NAN : inverse * times;
-        each([&](uint4 &x, int32_t j, int) {
-          if (j >= last) return;
-          float f[kPer<T>];
-          Unpack(x, f, span.row);
-#pragma unroll
-          for (int e = 0; e < kPer<T>; ++e) f[e] = Exp2((f[e] - from) * k) * spread;
-          Store(out, span, aligned, j, f);
-        });
-        TeamSync<kTeam>();
-        if (!teacher.wrong)
-          WriteNamed(rows, span.row, out, max(0, span.Column(first)),
-                     min(span.classes, span.Column(last)), t.entries, token, share, tid, kTeam,
-                     from, k, inverse, times);
-      }
     }
-    if (loss && rank == 0 && tid == 0)
-      loss[r] = row_loss * by.host.rounded;
+    if (out && !teacher.some) {
+      WriteZeros(out, rows.classes, zeros_first, zeros_last, tid, kTeam);
+    } else if (out) {
+      if (by.device) WaitForPrevious();
+      const float times = t.temperature * (by.device ? by.device->rounded : by.host.rounded);
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
+      const float spread = teacher.wrong ? NAN : inverse * times;
+      each([&](int i, int32_t j) {
+        if (j >= last) return;
+        float f[kPer<T>];
+        Spread(Packed(v[i]), span.row, from, k, spread, f);
+        Store(out, span, aligned, j, f);
+      });
+      __syncthreads();
+      if (!teacher.wrong)
+        WriteNamed(span.row, out, max(0, span.Column(first)),
+                   min(span.classes, span.Column(last)), t.entries, token, share, tid, kTeam,
+                   from, k, inverse, times);
+    }
   }
-  if (loss) return;
+  if (loss) {
+    if (rank == 0 && tid == 0) loss[r] = row_loss * by.host.rounded;
+    return;
+  }
   // (the next kernel reads the scale too, and waits for nothing but this one's end)
   if (by.device) WaitForPrevious();
-  if (kTeam == 32) {
-    if (lane == 0) losses[warp] = row_loss;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      double sum = 0.0;
-      for (uint32_t w = 0; w < blockDim.x / 32; ++w) sum += losses[w];
-      partial[blockIdx.x] = sum;
-    }
-  } else if (rank == 0 && tid == 0) {
-    partial[blockIdx.x / cluster] = row_loss;
-  }
+  if (rank == 0 && tid == 0) partial[r] = row_loss;
 }
 
 __global__ void __launch_bounds__(1024)
@@ -319,7 +427,7 @@ DistilLoss(const double *partial, int32_t parts, DistilBy by, float *loss) {
 }
 
 // The gradient for an upstream, of rows whose norm is known: `items` parts of rows (kTeam 256) or
-// eight rows (kTeam 32), dealt out to the blocks there are.  unless_one: what is there stays where
+// a row per warp (kTeam 32), dealt out to the blocks there are.  unless_one: what is there stays where
 // the upstream is 1.
 template <typename T, int kTeam>
 __global__ void __launch_bounds__(256, 4)
@@ -352,11 +460,11 @@ DistilBackward(Rows<T> rows, Teacher t, const float4 *norm, T *grad, int64_t out
                           rows.classes);
     const int32_t last = kTeam == 32 ? span.vectors : min(span.vectors, first + part);
     uint4 v[kTile];
-    LoadTile<kTeam, kTile>(v, span, first, last, tid);
+    LoadTile<kTeam, kTile>(v, span, rows, first, last, tid);
     TeacherRow teacher = {};
     if (kTeam == 32 || warp == 0) {
       teacher = ReadTeacher(t, r, rows.classes, lane, token, share);
-      ShareOut(t, teacher, k, lane, share);
+      ShareOut(t, teacher, span.row, k, 0.0f, lane, token, share);
       if (kTeam > 32 && lane == 0) {
         flags[0] = teacher.some;
         flags[1] = teacher.wrong;
@@ -378,21 +486,19 @@ DistilBackward(Rows<T> rows, Teacher t, const float4 *norm, T *grad, int64_t out
     const float spread = teacher.wrong ? NAN : inverse * times;
     const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
     for (int32_t tile = first; tile < last; tile += kTeam * kTile) {
-      if (tile != first) LoadTile<kTeam, kTile>(v, span, tile, last, tid);
+      if (tile != first) LoadTile<kTeam, kTile>(v, span, rows, tile, last, tid);
 #pragma unroll
       for (int i = 0; i < kTile; ++i) {
         const int32_t j = tile + i * kTeam + tid;
         if (j >= last) continue;
         float f[kPer<T>];
-        Unpack(Packed(v[i]), f, span.row);
-#pragma unroll
-        for (int e = 0; e < kPer<T>; ++e) f[e] = Exp2((f[e] - n.x) * k) * spread;
+        Spread(Packed(v[i]), span.row, n.x, k, spread, f);
         Store(out, span, aligned, j, f);
       }
     }
     TeamSync<kTeam>();
     if (!teacher.wrong)
-      WriteNamed(rows, span.row, out, max(0, span.Column(first)),
+      WriteNamed(span.row, out, max(0, span.Column(first)),
                  min(span.classes, span.Column(last)), t.entries, token, share, tid, kTeam, n.x,
                  k, inverse, times);
     TeamSync<kTeam>();  // the next row's entries come to the same place
@@ -451,22 +557,29 @@ int32_t LaunchDistil(const k2b200_class_rows *rows, const k2b200_teacher *t, flo
     NoteLaunch();
   }
   if (r.count > 0) {
-    auto kernel = p.team == 32    ? (p.vectors == 1   ? Distil<T, 32, 1, false>
-                                     : p.vectors == 2 ? Distil<T, 32, 2, false>
-                                     : p.vectors == 4 ? Distil<T, 32, 4, false>
-                                                      : Distil<T, 32, 8, false>)
-                  : p.team == 128 ? (p.vectors == 4 ? Distil<T, 128, 4, false>
-                                                    : Distil<T, 128, 8, false>)
-                  : p.again       ? Distil<T, 256, 16, true>
-                  : p.vectors == 4 ? Distil<T, 256, 4, false>
-                  : p.vectors == 8 ? Distil<T, 256, 8, false>
-                                   : Distil<T, 256, 16, false>;
-    const size_t smem = (sizeof(int32_t) + sizeof(float)) * t->entries *
-                        (p.team == 32 ? p.rows_per_block : 1);
-    K2B_CUDA_OK(LaunchRows(kernel, groups * p.cluster, p.block, smem, p.cluster,
-                           by.device != nullptr, s, r, teacher, reinterpret_cast<float4 *>(norm),
-                           t->reduction == 0 ? loss : nullptr, partial, static_cast<T *>(grad),
-                           outer_stride, inner_stride, by));
+    const size_t entry = sizeof(int32_t) + sizeof(float);
+    float4 *norms = reinterpret_cast<float4 *>(norm);
+    float *row_losses = t->reduction == 0 ? loss : nullptr;
+    if (p.team == 32) {
+      auto kernel = p.vectors == 1   ? DistilWarps<T, 1>
+                    : p.vectors == 2 ? DistilWarps<T, 2>
+                    : p.vectors == 4 ? DistilWarps<T, 4>
+                                     : DistilWarps<T, 8>;
+      K2B_CUDA_OK(LaunchRows(kernel, groups, p.block, entry * t->entries * (p.block / 32), 1,
+                             by.device != nullptr, s, r, teacher, norms, row_losses, partial,
+                             static_cast<T *>(grad), outer_stride, inner_stride, by,
+                             p.rows_per_warp));
+    } else {
+      auto kernel = p.team == 128   ? (p.vectors == 4 ? DistilBlocks<T, 128, 4, false>
+                                                      : DistilBlocks<T, 128, 8, false>)
+                    : p.again        ? DistilBlocks<T, 256, 16, true>
+                    : p.vectors == 4 ? DistilBlocks<T, 256, 4, false>
+                    : p.vectors == 8 ? DistilBlocks<T, 256, 8, false>
+                                     : DistilBlocks<T, 256, 16, false>;
+      K2B_CUDA_OK(LaunchRows(kernel, groups * p.cluster, p.block, entry * t->entries, p.cluster,
+                             by.device != nullptr, s, r, teacher, norms, row_losses, partial,
+                             static_cast<T *>(grad), outer_stride, inner_stride, by));
+    }
     NoteLaunch();
   }
   if (t->reduction != 0) {
@@ -490,13 +603,13 @@ int32_t LaunchDistilBackward(const k2b200_class_rows *rows, const k2b200_teacher
   // vectors of a row, wherever it begins, in parts of a block's four per thread
   const int32_t part = 1024, parts = CeilDiv((int64_t)r.classes + kPer<T> - 1, kPer<T>) + 1;
   const int32_t row_parts = p.team == 32 ? 1 : CeilDiv(parts, part);
-  const int64_t items = p.team == 32 ? CeilDiv(r.count, p.rows_per_block)
+  const int64_t items = p.team == 32 ? CeilDiv(r.count, p.block / 32)
                                      : (int64_t)r.count * row_parts;
   const int64_t blocks = std::min<int64_t>(items, 8 * (int64_t)NumSms());
   auto kernel = p.team == 32 ? DistilBackward<T, 32> : DistilBackward<T, 256>;
   const int32_t threads = p.team == 32 ? p.block : 256;
   const size_t smem =
-      (sizeof(int32_t) + sizeof(float)) * t->entries * (p.team == 32 ? p.rows_per_block : 1);
+      (sizeof(int32_t) + sizeof(float)) * t->entries * (p.team == 32 ? p.block / 32 : 1);
   kernel<<<(uint32_t)blocks, threads, smem, s>>>(
       r, teacher, reinterpret_cast<const float4 *>(norm), static_cast<T *>(grad), outer_stride,
       inner_stride, ByOf(rows, t, workspace), *up, unless_one, items, row_parts, part);
