@@ -1,11 +1,14 @@
 // Rows of class scores as the kernels of token_scores.cu and distillation.cu hold them.
 //
-// A row is read once, as aligned vectors of 16 bytes, into the registers of a team of threads: a
-// warp up to 4 KB, 128 threads up to 16, 256 up to 64, and a cluster of up to 8 such blocks up to
-// 512.  Where the row begins inside a vector (any alignment of an element will do) the elements of
-// the first and the last vector are read one by one, and what lies outside the row is -inf there.
-// What a kernel needs of the row more than once it takes from the registers.  Longer rows are read
-// again, tile by tile.
+// A team of threads - a warp, a block, or the blocks of a cluster - has a row at a time, as aligned
+// vectors of 16 bytes that each thread copies to shared memory for itself: no barrier stands between
+// a copy and its use, only cp.async's own wait, and other rows are on their way meanwhile.  Short
+// rows (up to 4 KB: a warp's 8 vectors per lane) go on to registers, and their place is free for the
+// warp's next row at once; longer ones are read from shared memory as often as they are needed, by
+// loops whose code stays in the instruction cache (unrolled over 20 vectors of a thread it did not:
+// 16000 x 5000 fp16 rows with their gradient took 120 us, most of it waiting for instructions).
+// Where a row begins inside a vector (any alignment of an element will do) the first and the last
+// vector are shared with its neighbours: what is not the row's is -inf.
 //
 //   p_c = 2^((x_c - high) * log2 e) / sum   high the largest score, sum over all classes
 //
@@ -18,6 +21,7 @@
 
 #include "../../include/k2b200.h"
 #include "common.cuh"
+#include "cp_async.cuh"
 
 namespace k2b {
 
@@ -126,6 +130,27 @@ __device__ __forceinline__ float ScoreOf(uint32_t order) {
 }
 __device__ __forceinline__ uint64_t KeyOf(float v, int32_t c) {
   return (uint64_t)OrderOf(v) << 32 | (uint32_t)~c;
+}
+
+__device__ __forceinline__ float WarpMaxF(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ float WarpSumF(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+// Both sums at once: the halves of the warp take one each.
+__device__ __forceinline__ float2 WarpSum2F(float a, float b) {
+  const bool high = threadIdx.x & 16;
+  float mine = high ? b : a;
+  mine += __shfl_xor_sync(0xffffffffu, high ? a : b, 16);
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  const float other = __shfl_xor_sync(0xffffffffu, mine, 16);
+  return high ? make_float2(other, mine) : make_float2(mine, other);
 }
 
 // ---------------------------------------------------------------------------
@@ -268,26 +293,28 @@ struct RowSpan {
       const int32_t c = c0 + k;
       f[k] = c >= 0 && c < classes ? ToFloat(row[c]) : -INFINITY;
     }
-    return Packed(f);  // (exact)
+    return Pack(f, row);  // (exact)
   }
   __device__ __forceinline__ uint4 Vector(int32_t j) const {
     const int32_t c0 = Column(j);
     return Whole(c0) ? *reinterpret_cast<const uint4 *>(row + c0) : Edge(j);
   }
-  __device__ __forceinline__ static uint4 Packed(const float (&f)[kPer<T>]) {
-    uint4 v = Pack(f, static_cast<const T *>(nullptr));
-    return k2b::Packed(v);
-  }
 };
 
 // Elements [begin, end) of a vector, -inf elsewhere.
-__device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end, const float *t) {
-  const uint4 low = LowestVector(t);
+__device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end, const float *t,
+                                      const uint4 &low) {
   return make_uint4(begin <= 0 && end > 0 ? v.x : low.x, begin <= 1 && end > 1 ? v.y : low.y,
                     begin <= 2 && end > 2 ? v.z : low.z, begin <= 3 && end > 3 ? v.w : low.w);
 }
+__device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end, const float *t) {
+  return Keep(v, begin, end, t, LowestVector(t));
+}
 template <typename T>
 __device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end, const T *t) {
+  // (whole words where pairs of scores are aligned)
+  if (((begin | end) & 1) == 0)
+    return Keep(v, begin / 2, end / 2, static_cast<const float *>(nullptr), LowestVector(t));
   // (a shift by 32 or more leaves nothing)
   const auto word = [&](uint32_t w, int32_t k, uint32_t low) {
     uint32_t from, to;
@@ -300,53 +327,97 @@ __device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end
   return make_uint4(word(v.x, 0, low), word(v.y, 1, low), word(v.z, 2, low), word(v.w, 3, low));
 }
 
-// Vectors tile + i * kTeam + tid for i < kVectors of those before `last`.  A vector that the row
-// shares with others is read as a whole where all of it lies between the first and the last class
-// of all rows, and element by element elsewhere.
+// A thread's vectors of a row: first + i * team for those before `last`, at slot[i * team].
+template <typename T>
+struct RowPart {
+  RowSpan<T> span;
+  int32_t first, last, mine;  // mine: this thread's
+  __device__ __forceinline__ RowPart(const RowSpan<T> &row, int32_t from, int32_t to, int32_t tid,
+                                     int32_t team)
+      : span(row), first(from + tid), last(to) {
+    mine = first < last ? (last - first + team - 1) / team : 0;
+  }
+};
+
+// Waits until what this thread has sent for is there.
+__device__ __forceinline__ void WaitForAll() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Sends for them.  A vector that the row shares with others is copied as a whole where all of it
+// lies between the first and the last class of all rows, and read element by element elsewhere.
+// kVectors: what a thread has at most (0: any number).
 template <int kTeam, int kVectors, typename T>
-__device__ __forceinline__ void LoadTile(uint4 (&v)[kVectors], const RowSpan<T> &span,
-                                         const Rows<T> &rows, int32_t tile, int32_t last,
-                                         int32_t tid) {
-  const int32_t end = span.vectors - 1, rest = span.classes - span.Column(end);
+__device__ __forceinline__ void SendFor(uint4 *slot, const RowPart<T> &part, const Rows<T> &rows) {
+  asm volatile("" ::: "memory");  // (behind the last use of what was there)
+  const RowSpan<T> &span = part.span;
+  const int32_t end = span.vectors - 1;
   const uint4 *at = reinterpret_cast<const uint4 *>(span.row - span.shift);
-  const bool front = span.shift != 0 && tile == 0,
-             tail = rest < kPer<T> && end >= tile && end < min(last, tile + kTeam * kVectors);
-  if ((!front || reinterpret_cast<const T *>(at) >= rows.begin) &&
-      (!tail || reinterpret_cast<const T *>(at + span.vectors) <= rows.end)) {
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int32_t j = tile + i * kTeam + tid;
-      v[i] = j < last ? at[j] : LowestVector(span.row);
-    }
-    if (front && tid == 0) v[0] = Keep(v[0], span.shift, kPer<T>, span.row);
-    if (tail) {
-      const int32_t slot = (end - tile) / kTeam;
-      const bool mine = ((end - tile) & (kTeam - 1)) == tid;
+  const bool front = reinterpret_cast<const T *>(at) >= rows.begin,
+             tail = reinterpret_cast<const T *>(at + span.vectors) <= rows.end;
+  if (front && tail) {
+    if (kVectors > 0) {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i)
-        if (i == slot) {
-          const uint4 kept = Keep(v[i], 0, rest, span.row);
-          if (mine) v[i] = kept;
-        }
+        if (i < part.mine) CpAsync16(slot + i * kTeam, at + part.first + i * kTeam);
+    } else {
+#pragma unroll 4
+      for (int32_t i = 0; i < part.mine; ++i)
+        CpAsync16(slot + i * kTeam, at + part.first + i * kTeam);
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int32_t j = tile + i * kTeam + tid;
-      v[i] = j < last && span.Whole(span.Column(j)) ? at[j] : LowestVector(span.row);
+    for (int32_t i = 0; i < part.mine; ++i) {
+      const int32_t j = part.first + i * kTeam;
+      if ((j > 0 || front) && (j < end || tail))
+        CpAsync16(slot + i * kTeam, at + j);
+      else
+        slot[i * kTeam] = span.Edge(j);
     }
-#pragma unroll 1
-    for (int32_t both = 0; both < 2; ++both) {
-      const int32_t j = both ? end : 0;
-      if (j < tile || j >= min(last, tile + kTeam * kVectors) ||
-          ((j - tile) & (kTeam - 1)) != tid || span.Whole(span.Column(j)))
-        continue;
-      const uint4 e = span.Edge(j);
-      const int32_t slot = (j - tile) / kTeam;
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-        if (i == slot) v[i] = e;
-    }
+  }
+}
+// The row behind the one at hand, whose vectors are sent for one by one, each as soon as its place
+// is free.  A row that SendFor would not copy as a whole waits for the end (Rest).
+template <int kTeam, typename T>
+struct Refill {
+  const uint4 *at;
+  int32_t mine;  // this thread's that are sent for one by one
+  __device__ __forceinline__ Refill(const RowPart<T> *part, const Rows<T> &rows)
+      : at(nullptr), mine(0) {
+    if (part == nullptr) return;
+    const RowSpan<T> &span = part->span;
+    const T *begin = span.row - span.shift;
+    if (begin < rows.begin || begin + (int64_t)span.vectors * kPer<T> > rows.end) return;
+    at = reinterpret_cast<const uint4 *>(begin) + part->first;
+    mine = part->mine;
+  }
+  __device__ __forceinline__ void operator()(uint4 *slot, int32_t i) const {
+    asm volatile("" ::: "memory");  // (behind the last use of what was there)
+    if (i < mine) CpAsync16(slot + i * kTeam, at + i * kTeam);
+  }
+  // What places `done` and on are for.
+  __device__ __forceinline__ void Rest(uint4 *slot, int32_t done, const RowPart<T> *part,
+                                       const Rows<T> &rows) const {
+    if (part == nullptr) return;
+    if (at == nullptr)
+      SendFor<kTeam, 0>(slot, *part, rows);
+    else
+      for (int32_t i = done; i < mine; ++i) (*this)(slot, i);
+  }
+};
+struct NoRefill {
+  __device__ __forceinline__ void operator()(uint4 *, int32_t) const {}
+};
+
+// -inf for what is not the row's, once they are there.
+template <int kTeam, typename T>
+__device__ __forceinline__ void CutEnds(uint4 *slot, const RowPart<T> &part) {
+  const RowSpan<T> &span = part.span;
+  const int32_t end = span.vectors - 1, rest = span.classes - span.Column(end);
+  if (span.shift != 0 && part.first == 0 && part.mine > 0)
+    slot[0] = Keep(slot[0], span.shift, kPer<T>, span.row);
+  if (rest < kPer<T> && part.mine > 0 && part.first + (part.mine - 1) * kTeam == end) {
+    uint4 &v = slot[(part.mine - 1) * kTeam];
+    v = Keep(v, 0, rest, span.row);
   }
 }
 
@@ -364,6 +435,113 @@ __device__ __forceinline__ void AddVector(const uint4 &v, const T *type, float h
   });
 }
 
+// A thread's vectors, from shared memory to registers.
+template <int kTeam, int kVectors, typename T>
+__device__ __forceinline__ void Take(uint4 (&v)[kVectors], const uint4 *slot,
+                                     const RowPart<T> &part) {
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i)
+    v[i] = i < part.mine ? slot[i * kTeam] : LowestVector(part.span.row);
+}
+
+// The largest score of a thread's vectors, those of the first and of the second half apart.
+template <int kVectors, typename T>
+__device__ __forceinline__ float2 Highest(uint4 (&v)[kVectors], const T *type) {
+  float half[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    float &g = half[2 * i / kVectors];
+    g = fmaxf(g, VectorMax(Packed(v[i]), type));
+  }
+  return make_float2(half[0], half[1]);
+}
+
+// Sums of 2^d and of d 2^d over a thread's vectors, d = (x - high) * k: two vectors at a time.
+template <bool kSlope, int kVectors, typename T>
+__device__ __forceinline__ float2 SumUp(uint4 (&v)[kVectors], const T *type, float high, float k) {
+  Two sum[2] = {}, slope[2] = {};
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    After(v[i], sum[i & 1]);
+    AddVector<kSlope>(v[i], type, high, k, sum[i & 1], slope[i & 1]);
+  }
+  const float2 s = Split(Add(sum[0], sum[1]));
+  if (!kSlope) return make_float2(s.x + s.y, 0.0f);
+  const float2 t = Split(Add(slope[0], slope[1]));
+  return make_float2(s.x + s.y, t.x + t.y);
+}
+
+// What a thread knows of a longer row's vectors: the largest score, of all and of every fourth
+// vector, and the sums of 2^d and d 2^d against it.
+struct Sums {
+  float high, group[4];
+  Two sum, slope;
+};
+__device__ __forceinline__ Sums NoSums() {
+  return {-INFINITY, {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, {0}, {0}};
+}
+// The sums so far, against a larger score.
+template <bool kSlope>
+__device__ __forceinline__ void Raise(Sums &s, float high, float k) {
+  if (!(high > s.high)) return;
+  const float d = fmaxf((s.high - high) * k, -1e30f), e = Exp2(d);
+  const Two by = MakeTwo(e, e);
+  if (kSlope) s.slope = Mul(by, Fma(s.sum, MakeTwo(d, d), s.slope));
+  s.sum = Mul(s.sum, by);
+  s.high = high;
+}
+// then(slot, i): called behind the last use of vector i.
+template <bool kSlope, int kTeam, typename T, typename F>
+__device__ __forceinline__ void AddRow(Sums &s, uint4 *slot, int32_t mine, const T *type, float k,
+                                       const F &then) {
+  int32_t i = 0;
+#pragma unroll 1
+  for (; i + 4 <= mine; i += 4) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      v[u] = slot[(i + u) * kTeam];
+      s.group[u] = fmaxf(s.group[u], VectorMax(v[u], type));
+    }
+    Raise<kSlope>(s, fmaxf(fmaxf(s.group[0], s.group[1]), fmaxf(s.group[2], s.group[3])), k);
+    const float from = s.high == -INFINITY ? 0.0f : s.high;
+    Two sum = {0}, slope = {0};  // of every second vector
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      After(v[u], u & 1 ? sum : s.sum);
+      AddVector<kSlope>(v[u], type, from, k, u & 1 ? sum : s.sum, u & 1 ? slope : s.slope);
+    }
+    s.sum = Add(s.sum, sum);
+    if (kSlope) s.slope = Add(s.slope, slope);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) then(slot, i + u);
+  }
+#pragma unroll 1
+  for (; i < mine; ++i) {
+    const uint4 v = slot[i * kTeam];
+    const float high = VectorMax(v, type);
+    // (as many groups as there are: a loop does not choose a register)
+    s.group[0] = (i & 3) == 0 ? fmaxf(s.group[0], high) : s.group[0];
+    s.group[1] = (i & 3) == 1 ? fmaxf(s.group[1], high) : s.group[1];
+    s.group[2] = (i & 3) == 2 ? fmaxf(s.group[2], high) : s.group[2];
+    Raise<kSlope>(s, high, k);
+    AddVector<kSlope>(v, type, s.high == -INFINITY ? 0.0f : s.high, k, s.sum, s.slope);
+    then(slot, i);
+  }
+}
+// A warp's sums against its largest score.
+template <bool kSlope>
+__device__ __forceinline__ float2 WarpSums(const Sums &s, float k, float *high) {
+  *high = WarpMaxF(s.high);
+  const float from = *high == -INFINITY ? 0.0f : *high;
+  const float d = (s.high - from) * k, e = Exp2(d);
+  const float2 sum = Split(s.sum);
+  if (!kSlope) return make_float2(WarpSumF((sum.x + sum.y) * e), 0.0f);
+  const float2 slope = Split(s.slope);
+  return WarpSum2F((sum.x + sum.y) * e,
+                   e * fmaf(sum.x + sum.y, fmaxf(d, -1e30f), slope.x + slope.y));
+}
+
 // Values for the classes of vector j into another row of the same length; `aligned`: both rows
 // begin at the same place of a vector.
 template <typename T>
@@ -379,41 +557,24 @@ __device__ __forceinline__ void Store(T *out, const RowSpan<T> &span, bool align
     if (c0 + k >= 0 && c0 + k < span.classes) out[c0 + k] = FromFloat<T>(f[k]);
 }
 
+// Zeros for a row.
+template <typename T>
+__device__ __forceinline__ void WriteZeros(T *out, int32_t classes, int32_t first, int32_t last,
+                                           int32_t tid, int32_t team) {
+  const RowSpan<T> zeros(out, classes);
+  const float f[kPer<T>] = {};
+  for (int32_t j = first + tid; j < min(last, zeros.vectors); j += team)
+    Store(out, zeros, true, j, f);
+}
+
 // ---------------------------------------------------------------------------
 // teams
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float WarpMaxF(float v) {
-  float m;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
-  return m;
-}
-__device__ __forceinline__ float WarpSumF(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
-}
-// Both sums at once: the halves of the warp take one each.
-__device__ __forceinline__ float2 WarpSum2F(float a, float b) {
-  const bool high = threadIdx.x & 16;
-  float mine = high ? b : a;
-  mine += __shfl_xor_sync(0xffffffffu, high ? a : b, 16);
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  const float other = __shfl_xor_sync(0xffffffffu, mine, 16);
-  return high ? make_float2(other, mine) : make_float2(mine, other);
-}
-
-// Blocks of an SM that a kernel is compiled for: the registers are the row's and some 40 more.
-constexpr int MinBlocks(int team, int vectors) {
-  return (vectors >= 16 ? 2 : vectors >= 8 ? 3 : 4) * (team == 128 ? 2 : 1);
-}
-
-// Adds sums of 2^d and d 2^d whose d is by `by` * log2 e too high (-inf: there are none).
-__device__ __forceinline__ void Join(float &sum, float &slope, float more, float more_slope,
-                                     float by) {
-  const float d = by * kLog2e, e = Exp2(d);
-  sum = fmaf(more, e, sum);
-  slope = fmaf(e, fmaf(more, fmaxf(d, -1e30f), more_slope), slope);
+// Sums that the lanes have against a score of their own (-inf: none), against the largest of them.
+__device__ __forceinline__ float2 JoinWarp(float h, float2 sums, float *high) {
+  *high = WarpMaxF(h);
+  const float d = (h - (*high == -INFINITY ? 0.0f : *high)) * kLog2e, e = Exp2(d);
+  return WarpSum2F(sums.x * e, e * fmaf(sums.x, fmaxf(d, -1e30f), sums.y));
 }
 
 template <int kTeam>
@@ -463,44 +624,69 @@ __device__ __forceinline__ V ReadFrom(const V *mine, uint32_t rank) {
 // ---------------------------------------------------------------------------
 // How the rows of a call are dealt out.
 struct RowPlan {
-  int32_t team;     // threads per row and block: 32, 128, 256
-  int32_t vectors;  // per thread
-  int32_t cluster;  // blocks per row
-  bool again;       // the row does not fit and is read again
-  int32_t block;    // threads of a block: `team`, or several warps that are a team each
-  int32_t rows_per_warp, rows_per_block;
+  int32_t team;       // threads per row and block: 32, 256 or 512
+  int32_t vectors;    // per thread: of a short row 1, 2, 4 or 8, which are registers; at most of others
+  bool in_registers;
+  int32_t cluster;    // blocks per row
+  int32_t tiles;      // parts of a row that does not fit: read again for each pass
+  int32_t block;      // threads of a block: a team, or several warps that are a team each
+  int32_t ring;       // bytes of a block's rows
+  int64_t blocks;     // what the device holds at a time, or what the rows need
 };
 
+// Blocks of an SM that the kernels for short rows are compiled for.
+constexpr int ResidentBlocks(int vectors) { return vectors > 4 ? 6 : 8; }
+
+// `more`: bytes of shared memory that a team takes besides.
 template <typename T>
-static inline RowPlan PlanRows(const Rows<T> &r) {
-  RowPlan p = {32, 1, 1, false, 32, 1, 1};
+static inline RowPlan PlanRows(const Rows<T> &r, int32_t more) {
+  RowPlan p = {32, 1, true, 1, 1, 32, 0, 0};
   const int64_t rows = r.count, size = sizeof(T);
   // its vectors: one more where it does not begin with one
   const bool whole = ((uintptr_t)r.scores | (uint64_t)(r.outer_stride * size) |
                       (uint64_t)(r.inner_stride * size)) % 16 == 0;
-  const int64_t bytes = r.classes * size + (whole ? 0 : 16 - size);
+  const int64_t vectors = (r.classes * size + (whole ? 0 : 16 - size) + 15) / 16;
   const int32_t sms = NumSms();
-  if (bytes <= 32 * 8 * 16) {
-    while (bytes > 32 * 16 * p.vectors) p.vectors *= 2;
-    // few rows: one to a warp, and warps to as many SMs as there are; many: four to a warp
-    p.rows_per_warp = rows >= 16 * 4 * (int64_t)sms ? 4 : 1;
+  constexpr int64_t kShared = 224 << 10;  // of an SM
+  int64_t fit;
+  if (vectors <= 32 * 8) {
+    while (vectors > 32 * p.vectors) p.vectors *= 2;
     p.block = 32 * (int32_t)std::min<int64_t>(4, std::max<int64_t>(1, rows / sms));
-    p.rows_per_block = p.block / 32 * p.rows_per_warp;
-    return p;
+    fit = (int64_t)ResidentBlocks(p.vectors) * (128 / p.block);
+  } else {
+    p.in_registers = false;
+    if (vectors <= 32 * 32 && rows >= 4 * (int64_t)sms) {
+      p.block = 128;
+    } else {
+      p.team = p.block = 256;
+      // over more SMs: rows that do not fit one, and few rows, down to 8 KB each
+      while (p.cluster < 8 && (vectors * 16 > p.cluster * kShared * 7 / 8 ||
+                               (rows * p.cluster * 2 <= sms && vectors > p.cluster * 2 * 512))) {
+        p.cluster *= 2;
+        p.team = p.block = 512;
+      }
+    }
+    const int64_t threads = (int64_t)p.cluster * p.team;
+    int64_t each = (vectors + threads - 1) / threads;
+    const int64_t most = kShared * 7 / 8 / 16 / p.team;
+    p.tiles = (int32_t)((each + most - 1) / most);
+    p.vectors = (int32_t)std::min(each, most);
+    fit = 2048 / p.block;
   }
-  p.team = p.block = bytes <= 128 * 8 * 16 ? 128 : 256;
-  if (p.team == 128) {
-    p.vectors = bytes <= 128 * 4 * 16 ? 4 : 8;
-    return p;
-  }
-  while (p.cluster < 8 && bytes > (int64_t)p.cluster * 256 * 16 * 16) p.cluster *= 2;
-  // few rows: over more SMs, down to 8 KB of the row each
-  while (p.cluster < 8 && rows * p.cluster * 2 <= sms && bytes > (int64_t)p.cluster * 2 * 8192)
-    p.cluster *= 2;
-  p.vectors = 4;
-  while (p.vectors < 16 && bytes > (int64_t)p.cluster * 256 * 16 * p.vectors) p.vectors *= 2;
-  p.again = bytes > (int64_t)p.cluster * 256 * 16 * p.vectors;
+  const int64_t teams = p.block / p.team;
+  p.ring = p.block * p.vectors * 16;
+  fit = std::min(fit, kShared / (p.ring + more * teams + 1024));
+  p.blocks = std::min<int64_t>((rows + teams - 1) / teams * p.cluster,
+                               sms * std::max<int64_t>(1, fit) / p.cluster * p.cluster);
   return p;
+}
+
+// Lets a kernel have more shared memory than the 48 KB that it has without asking (of which the
+// kernels here name up to 17 themselves).
+template <typename... Params>
+static cudaError_t AllowShared(void (*kernel)(Params...), size_t bytes) {
+  if (bytes <= 30 << 10) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
 // A launch of `blocks` blocks in clusters; `behind`: see LaunchBehind (common.cuh).

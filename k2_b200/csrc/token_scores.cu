@@ -32,7 +32,7 @@ static inline int32_t RoomFor(int32_t top_k) {
 constexpr uint32_t kOrderOfNone = 0x007fffffu;  // OrderOf(-inf)
 
 // The largest bound found that at least k of a warp's kGroups values per lane reach, where there
-// are so many; -inf else.  By bisection, until no more than a quarter too many reach it.
+// are so many; -inf else.  By bisection, until no more than an eighth too many reach it.
 template <int kGroups>
 __device__ __forceinline__ uint32_t BoundOf(const uint32_t (&order)[kGroups], int32_t k) {
   uint32_t least = order[0], most = order[0];
@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t BoundOf(const uint32_t (&order)[kGroups], in
     for (int g = 0; g < kGroups; ++g) reach += __popc(__ballot_sync(0xffffffffu, order[g] >= mid));
     if (reach >= k) {
       low = mid;
-      if (reach <= k + (k >> 2)) break;
+      if (reach <= k + (k >> 3)) break;
     } else {
       high = mid;
     }
@@ -59,34 +59,95 @@ __device__ __forceinline__ uint32_t BoundOf(const uint32_t (&order)[kGroups], in
   return low;
 }
 
-// Whether scores of a thread's vectors are below `least`: bit 31 - k % 32 of word k / 32 for score k
-// of them (NaN is not).  The sign of a difference is shifted in, one instruction a score and half a
-// one for the difference.
-template <typename T, int kVectors>
-struct Below {
-  static constexpr int kScores = kVectors * kPer<T>, kWords = (kScores + 31) / 32,
-                       kEmpty = kWords * 32 - kScores;
-  uint32_t word[kWords];
-  __device__ __forceinline__ Below(uint4 (&v)[kVectors], const T *type, float least) {
-    const float up = 0.0f - least;  // (+0 for both zeros: neither is below the other)
-    const Two minus = MakeTwo(up, up);
+// Bit e is set where score e of a vector is not below `least` (NaN is not).
+__device__ __forceinline__ uint32_t Reaching(const uint4 &v, float least, const float *) {
+  return (!(__uint_as_float(v.x) < least) ? 1u : 0u) | (!(__uint_as_float(v.y) < least) ? 2u : 0u) |
+         (!(__uint_as_float(v.z) < least) ? 4u : 0u) | (!(__uint_as_float(v.w) < least) ? 8u : 0u);
+}
+template <typename Pair>
+__device__ __forceinline__ uint32_t ReachingPairs(const uint4 &v, Pair least) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t bits = 0;
 #pragma unroll
-    for (int w = 0; w < kWords; ++w) word[w] = 0;
+  for (int k = 0; k < 4; ++k) {
+    Pair p;
+    memcpy(&p, &w[k], 4);
+    // all bits of a half that reaches: of the low one bit 2k, of the high one bit 16 + 2k + 1
+    bits |= __hgeu2_mask(p, least) & ((1u << 2 * k) | (1u << (17 + 2 * k)));
+  }
+  return (bits | bits >> 16) & 0xff;
+}
+__device__ __forceinline__ uint32_t Reaching(const uint4 &v, float least, const __half *) {
+  return ReachingPairs(v, __half2half2(__float2half_rd(least)));
+}
+__device__ __forceinline__ uint32_t Reaching(const uint4 &v, float least, const __nv_bfloat16 *) {
+  return ReachingPairs(v, __bfloat162bfloat162(__float2bfloat16_rd(least)));
+}
+
+// One more of what a team counts in shared memory; few lanes come here at a time, so that nothing is
+// gained by adding theirs up first.
+__device__ __forceinline__ int32_t Count(int32_t *found) {
+  int32_t at;
+  asm volatile("atom.shared.add.u32 %0, [%1], 1;"
+               : "=r"(at)
+               : "r"((uint32_t)__cvta_generic_to_shared(found))
+               : "memory");
+  return at;
+}
+
+// Puts the keys of a thread's scores that reach `least` where there is room, counting them all.  A
+// score's vector is told by its bit, but no register by a number: it is read again, from the cache.
+template <int kTeam, int kVectors, typename T>
+__device__ __forceinline__ void Collect(uint4 (&v)[kVectors], const RowPart<T> &part, float least,
+                                        uint64_t *keys, int32_t room, int32_t *found) {
+  constexpr int kWord = 32 / kPer<T>;  // vectors to a word of bits
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      EachPair(Packed(v[i]), type, [&](float2 x, int) {
-        const float2 d = Split(Add(MakeTwo(x.x, x.y), minus));
-        uint32_t &w = word[i * kPer<T> / 32];
-        w = __funnelshift_l(__float_as_uint(d.x), w, 1);
-        w = __funnelshift_l(__float_as_uint(d.y), w, 1);
-      });
-    word[kWords - 1] <<= kEmpty;
+  for (int i0 = 0; i0 < kVectors; i0 += kWord) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int u = 0; u < kWord && i0 + u < kVectors; ++u)
+      bits |= Reaching(Packed(v[i0 + u]), least, part.span.row) << (u * kPer<T>);
+    while (bits) {
+      const int32_t bit = __ffs(bits) - 1;
+      bits &= bits - 1;
+      const int32_t i = i0 + bit / kPer<T>,
+                    c = part.span.Column(part.first + i * kTeam) + bit % kPer<T>;
+      // (beside the row there is nothing but -inf)
+      if (i >= part.mine || c < 0 || c >= part.span.classes) continue;
+      const uint64_t key = KeyOf(ToFloat(part.span.row[c]), c);
+      const int32_t at = Count(found);
+      if (at < room) keys[at] = key;
+    }
   }
-  // The scores that are not, of word w.
-  __device__ __forceinline__ uint32_t Not(int w) const {
-    return ~word[w] & (w + 1 == kWords ? ~0u << kEmpty : ~0u);
+}
+
+// The same for a thread's vectors in shared memory, where a score is read by its number.
+template <int kTeam, typename T, typename F>
+__device__ __forceinline__ void CollectRow(uint4 *slot, const RowPart<T> &part, float least,
+                                           uint64_t *keys, int32_t room, int32_t *found,
+                                           const F &then) {
+  constexpr int kWord = 32 / kPer<T>;
+#pragma unroll 1
+  for (int32_t i0 = 0; i0 < part.mine; i0 += kWord) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int u = 0; u < kWord; ++u)
+      if (i0 + u < part.mine)
+        bits |= Reaching(slot[(i0 + u) * kTeam], least, part.span.row) << (u * kPer<T>);
+    while (bits) {
+      const int32_t bit = __ffs(bits) - 1, i = i0 + bit / kPer<T>, e = bit % kPer<T>;
+      bits &= bits - 1;
+      const int32_t c = part.span.Column(part.first + i * kTeam) + e;
+      // (beside the row there is nothing but -inf)
+      if (c < 0 || c >= part.span.classes) continue;
+      const int32_t at = Count(found);
+      if (at < room) keys[at] = KeyOf(ToFloat(reinterpret_cast<const T *>(slot + i * kTeam)[e]), c);
+    }
+#pragma unroll
+    for (int u = 0; u < kWord; ++u)
+      if (i0 + u < part.mine) then(slot, i0 + u);
   }
-};
+}
 
 // Keys of a row's classes [first, last) vectors by a team, read from memory: of those that reach
 // `bound` the number, or each of them.
@@ -160,398 +221,423 @@ __device__ __forceinline__ void SkipTop(const TokenOut &out, int32_t r, int32_t 
   }
 }
 
-// Rows of up to 4 KB: a warp takes `per_warp` of them one after the other.  Lane q knows where the
-// q-th of them is and its given class, gathers its sums, and computes what a row has one of, for
-// all rows of the warp at once.
+// The places of n keys among them, for those of the top: rank by counting.
+template <typename F>
+__device__ __forceinline__ void EachPlace(const uint64_t *keys, int32_t n, int32_t tid,
+                                          int32_t team, F &&f) {
+  for (int32_t k = tid; k < n; k += team) {
+    const uint64_t key = keys[k];
+    int32_t place = 0;
+#pragma unroll 4
+    for (int32_t o = 0; o < n; ++o) place += keys[o] > key;
+    f(place, key);
+  }
+}
+
+// Short rows: each warp is a team.  It takes 32 rows at a time, a whole grid of warps apart; lane q
+// knows where the q-th of them is and its given class, gathers its sums, and computes what a row
+// has one of, for all of them at once.
 template <typename T, int kVectors, bool kTop>
-__global__ void __launch_bounds__(128, kVectors >= 8 ? 6 : 8)
-TokenWarps(Rows<T> rows, TokenOut out, int32_t per_warp) {
-  extern __shared__ uint64_t all_keys[];
-  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t *keys = all_keys + warp * out.room;
-  const int32_t first = (int32_t)(blockIdx.x * (blockDim.x >> 5) + warp) * per_warp,
-                mine = first + lane, taken = min(per_warp, rows.count - first);
-  if (taken <= 0) return;
-  const T *my_row = nullptr;
-  int64_t token = -1;
-  float score = 0.0f, my_high = 0.0f, my_sum = 0.0f, my_slope = 0.0f;
-  if (lane < taken) {
-    const RowPlace at = PlaceOf(rows, mine);
-    if (at.counts) {
-      my_row = rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride;
-      if (out.log_probs) {
-        token = IntAt(out.tokens, out.tokens_64, mine);
-        if (token >= 0 && token < rows.classes) score = ToFloat(my_row[token]);
-      }
-    }
-  }
+__global__ void __launch_bounds__(128, ResidentBlocks(kVectors))
+TokenWarps(Rows<T> rows, TokenOut out) {
+  extern __shared__ uint4 shared[];
+  __shared__ int32_t all_found[4];
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  uint4 *slot = shared + warp * 32 * kVectors + lane;
+  uint64_t *keys = reinterpret_cast<uint64_t *>(shared + warps * 32 * kVectors) + warp * out.room;
+  const int32_t apart = (int32_t)gridDim.x * warps;
   const bool slopes = out.entropy || out.norm;
-  for (int32_t q = 0; q < taken; ++q) {
-    const T *row = reinterpret_cast<const T *>(
-        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(my_row), q));
-    if (row == nullptr) {
-      if (kTop) SkipTop(out, first + q, lane, 32);
-      continue;
-    }
-    const RowSpan<T> span(row, rows.classes);
-    uint4 v[kVectors];
-    LoadTile<32, kVectors>(v, span, rows, 0, span.vectors, lane);
-    // the largest score, of the warp and of two groups per lane
-    float group[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      float &g = group[2 * i / kVectors];
-      g = fmaxf(g, VectorMax(Packed(v[i]), span.row));
-    }
-    const float lane_high = fmaxf(group[0], group[1]), high = WarpMaxF(lane_high),
-                from = high == -INFINITY ? 0.0f : high;
-    // the sums, of two vectors at a time
-    Two sums[2] = {}, slope[2] = {};
-    if (slopes) {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        After(v[i], sums[i & 1]);
-        AddVector<true>(v[i], span.row, from, kLog2e, sums[i & 1], slope[i & 1]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        After(v[i], sums[i & 1]);
-        AddVector<false>(v[i], span.row, from, kLog2e, sums[i & 1], slope[i & 1]);
-      }
-    }
-    const float2 s = Split(Add(sums[0], sums[1])), t = Split(Add(slope[0], slope[1]));
-    const float2 both =
-        slopes ? WarpSum2F(s.x + s.y, t.x + t.y) : make_float2(WarpSumF(s.x + s.y), 0.0f);
-    const float sum = both.x;
-    if (lane == q) {
-      my_high = from;
-      my_sum = sum;
-      my_slope = both.y;
-    }
-    if (kTop) {
-      float least;
-      if (out.top_k <= 16) {
-        // the k-th of the lanes' largest: take away the largest k times, whoever has it
-        float left = lane_high;
-        least = high;
-        for (int32_t k = 1; k < out.top_k; ++k) {
-          if (left == least) left = -INFINITY;
-          least = WarpMaxF(left);
+  for (int32_t base = (int32_t)blockIdx.x * warps + warp; base < rows.count; base += 32 * apart) {
+    const int32_t mine = base + lane * apart,
+                  taken = min(32, (rows.count - base + apart - 1) / apart);
+    const T *my_row = nullptr;
+    int64_t token = -1;
+    float score = 0.0f, my_high = 0.0f, my_sum = 0.0f, my_slope = 0.0f;
+    if (lane < taken) {
+      const RowPlace at = PlaceOf(rows, mine);
+      if (at.counts) {
+        my_row = rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride;
+        if (out.log_probs) {
+          token = IntAt(out.tokens, out.tokens_64, mine);
+          if (token >= 0 && token < rows.classes) score = ToFloat(my_row[token]);
         }
+      }
+    }
+    const auto row_of = [&](int32_t q) {
+      return reinterpret_cast<const T *>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(my_row), q & 31));
+    };
+    const T *next = row_of(0);
+    if (next != nullptr) {
+      const RowSpan<T> span(next, rows.classes);
+      SendFor<32, kVectors>(slot, RowPart<T>(span, 0, span.vectors, lane, 32), rows);
+    }
+    for (int32_t q = 0; q < taken; ++q) {
+      const T *row = next;
+      const RowSpan<T> span(row, rows.classes);
+      const RowPart<T> part(span, 0, span.vectors, lane, 32);
+      uint4 v[kVectors];
+      if (row != nullptr) {
+        WaitForAll();
+        CutEnds<32>(slot, part);
+        Take<32, kVectors>(v, slot, part);
+      }
+      next = row_of(q + 1);
+      if (q + 1 < taken && next != nullptr) {
+        const RowSpan<T> coming(next, rows.classes);
+        SendFor<32, kVectors>(slot, RowPart<T>(coming, 0, coming.vectors, lane, 32), rows);
+      }
+      if (row == nullptr) {
+        if (kTop) SkipTop(out, base + q * apart, lane, 32);
+        continue;
+      }
+      const float2 half = Highest(v, row);
+      const float high = WarpMaxF(fmaxf(half.x, half.y)), from = high == -INFINITY ? 0.0f : high;
+      float2 both;
+      if (slopes) {
+        const float2 s = SumUp<true>(v, row, from, kLog2e);
+        both = WarpSum2F(s.x, s.y);
       } else {
-        const uint32_t two[2] = {OrderOf(group[0]), OrderOf(group[1])};
-        least = ScoreOf(BoundOf(two, out.top_k));
+        both = make_float2(WarpSumF(SumUp<false>(v, row, from, kLog2e).x), 0.0f);
       }
-      const Below<T, kVectors> below(v, span.row, least);
-      int32_t found = 0;
-      __syncwarp();  // (the keys of the row before have been read)
-#pragma unroll
-      for (int w = 0; w < below.kWords; ++w) {
-        uint32_t hits = below.Not(w);
-        // each lane's hits one after the other; its scores come from a cache again
-        for (uint32_t some; (some = __ballot_sync(0xffffffffu, hits != 0)) != 0;) {
-          uint64_t key = 0;
-          if (hits) {
-            const int32_t bit = __clz(hits), k = 32 * w + bit;
-            hits &= ~(0x80000000u >> bit);
-            const int32_t c = span.Column(k / kPer<T> * 32 + lane) + k % kPer<T>;
-            if (c >= 0 && c < span.classes) key = KeyOf(ToFloat(row[c]), c);
+      const float sum = both.x;
+      if (lane == q) {
+        my_high = from;
+        my_sum = sum;
+        my_slope = both.y;
+      }
+      if (kTop) {
+        float least;
+        if (out.top_k <= 16) {
+          // the k-th of the lanes' largest: take away the largest k times, whoever has it
+          float left = fmaxf(half.x, half.y);
+          least = high;
+          for (int32_t k = 1; k < out.top_k; ++k) {
+            if (left == least) left = -INFINITY;
+            least = WarpMaxF(left);
           }
-          const uint32_t good = __ballot_sync(0xffffffffu, key != 0);
-          const int32_t place = found + __popc(good & ((1u << lane) - 1));
-          if (key != 0 && place < out.room) keys[place] = key;
-          found += __popc(good);
+        } else {
+          const uint32_t two[2] = {OrderOf(half.x), OrderOf(half.y)};
+          least = ScoreOf(BoundOf(two, out.top_k));
         }
-      }
-      __syncwarp();
-      if (found > out.room) {
-        const uint64_t bound = RaiseBound(
-            (uint64_t)OrderOf(least) << 32, out.top_k, out.room, span.classes,
-            [&](uint64_t key) {
-              int32_t n = 0;
-              EachKey<32>(span, 0, span.vectors, lane, key, [&](uint64_t) { ++n; });
-              return (int32_t)__reduce_add_sync(0xffffffffu, n);
-            });
-        // (a key's place among those of the lane's and of lower lanes')
-        int32_t n = 0;
-        EachKey<32>(span, 0, span.vectors, lane, bound, [&](uint64_t) { ++n; });
-        int32_t place = n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int32_t o = __shfl_up_sync(0xffffffffu, place, d);
-          if (lane >= d) place += o;
-        }
-        found = __shfl_sync(0xffffffffu, place, 31);
-        place -= n;
-        EachKey<32>(span, 0, span.vectors, lane, bound,
-                    [&](uint64_t key) { keys[place++] = key; });
+        if (lane == 0) all_found[warp] = 0;
+        __syncwarp();  // (and the keys of the row before have been read)
+        Collect<32>(v, part, least, keys, out.room, &all_found[warp]);
         __syncwarp();
-      }
-      const float log_sum = logf(sum);
-      for (int32_t k = lane; k < found; k += 32) {
-        const uint64_t key = keys[k];
-        int32_t place = 0;
-        for (int32_t o = 0; o < found; ++o) place += keys[o] > key;
-        if (place < out.top_k) WriteTop(out, first + q, place, key, from, sum, log_sum);
+        int32_t found = all_found[warp];
+        if (found > out.room) {
+          const uint64_t bound = RaiseBound(
+              (uint64_t)OrderOf(least) << 32, out.top_k, out.room, span.classes,
+              [&](uint64_t key) {
+                int32_t n = 0;
+                EachKey<32>(span, 0, span.vectors, lane, key, [&](uint64_t) { ++n; });
+                return (int32_t)__reduce_add_sync(0xffffffffu, n);
+              });
+          __syncwarp();
+          if (lane == 0) all_found[warp] = 0;
+          __syncwarp();
+          EachKey<32>(span, 0, span.vectors, lane, bound,
+                      [&](uint64_t key) { keys[atomicAdd(&all_found[warp], 1)] = key; });
+          __syncwarp();
+          found = all_found[warp];
+        }
+        const float log_sum = logf(sum);
+        EachPlace(keys, found, lane, 32, [&](int32_t place, uint64_t key) {
+          if (place < out.top_k)
+            WriteTop(out, base + q * apart, place, key, from, sum, log_sum);
+        });
       }
     }
-  }
-  if (lane < taken) {
-    if (my_row != nullptr)
-      Finish(out, mine, rows.classes, token, score, my_high, my_sum, my_slope);
-    else
-      SkipRow(out, mine);
+    if (lane < taken) {
+      if (my_row != nullptr)
+        Finish(out, mine, rows.classes, token, score, my_high, my_sum, my_slope);
+      else
+        SkipRow(out, mine);
+    }
   }
 }
 
 template <int kTeam>
 struct TokenShared {
-  float high[kTeam / 32];
-  float2 sums[kTeam / 32];
+  float high[2][kTeam / 32];
+  float2 sums[2][kTeam / 32];
   int32_t counted[kTeam / 32];
   int32_t found;
   uint32_t bound;
-  float group[2 * kTeam];
+  float all_high;  // of a block, for its cluster
+  float2 all_sums;
+  float group[kTeam == 32 ? 1 : 4 * kTeam];
 };
 
-// What the blocks of a cluster tell each other.
-struct TokenCluster {
-  float high, sum, slope;
+// The keys that the blocks of a cluster show each other.
+struct TokenTogether {
   int32_t top;                       // keys in `list`
   uint64_t list[K2B200_MAX_TOP];     // this block's, largest first
-  uint64_t others[8 * K2B200_MAX_TOP];
+  uint64_t others[7 * K2B200_MAX_TOP];
 };
 
-// A block of kTeam threads per row with kVectors vectors each; kAgain: the row does not fit and is
-// read again for each pass.  Rows of a cluster of blocks (kTeam 256) are dealt out in slices.
-template <typename T, int kTeam, int kVectors, bool kTop, bool kAgain>
-__global__ void __launch_bounds__(kTeam, MinBlocks(kTeam, kVectors))
-TokenBlocks(Rows<T> rows, TokenOut out) {
-  extern __shared__ uint64_t keys[];
-  __shared__ TokenShared<kTeam> sh;
-  // (the smallest where blocks share no row)
-  __shared__ typename std::conditional<kTeam == 256, TokenCluster, int32_t>::type together;
-  const int32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t cluster = kTeam == 256 ? ClusterSize() : 1,
-                 rank = kTeam == 256 ? ClusterRank() : 0;
-  const int32_t r = (int32_t)(blockIdx.x / cluster);
-  const RowPlace at = PlaceOf(rows, r);
-  if (!at.counts) {
-    if (rank == 0) {
-      if (tid == 0) SkipRow(out, r);
-      SkipTop(out, r, tid, kTeam);
-    }
-    return;  // (all blocks of the cluster)
-  }
-  const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
-                        rows.classes);
-  const int32_t slice = (span.vectors + (int32_t)cluster - 1) / (int32_t)cluster;
-  const int32_t first = min(span.vectors, (int32_t)rank * slice),
-                last = min(span.vectors, first + slice);
-
-  uint4 v[kVectors];
-  const auto each = [&](auto &&f) {
-    if constexpr (kAgain) {
-      for (int32_t tile = first; tile < last; tile += kTeam * kVectors) {
-        LoadTile<kTeam, kVectors>(v, span, rows, tile, last, tid);
-#pragma unroll
-        for (int i = 0; i < kVectors; ++i) f(i);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) f(i);
-    }
-  };
-  if (!kAgain) LoadTile<kTeam, kVectors>(v, span, rows, first, last, tid);
-  // the given class's score is on its way meanwhile
-  int64_t token = -1;
-  float token_score = 0.0f;
-  if (out.log_probs && tid == 0 && rank == 0) {
-    token = IntAt(out.tokens, out.tokens_64, r);
-    if (token >= 0 && token < rows.classes) token_score = ToFloat(span.row[token]);
-  }
-
-  // the largest score, of the warp and of two groups per thread; the warp's sums
-  float group[2] = {-INFINITY, -INFINITY};
-  each([&](int i) {
-    float &g = group[2 * i / kVectors];
-    g = fmaxf(g, VectorMax(Packed(v[i]), span.row));
-  });
-  const float warp_high = WarpMaxF(fmaxf(group[0], group[1])),
-              warp_from = warp_high == -INFINITY ? 0.0f : warp_high;
-  Two sums[2] = {}, slopes[2] = {};
-  if (out.entropy || out.norm)
-    each([&](int i) {
-      After(v[i], sums[i & 1]);
-      AddVector<true>(v[i], span.row, warp_from, kLog2e, sums[i & 1], slopes[i & 1]);
-    });
-  else
-    each([&](int i) {
-      After(v[i], sums[i & 1]);
-      AddVector<false>(v[i], span.row, warp_from, kLog2e, sums[i & 1], slopes[i & 1]);
-    });
-  const float2 s = Split(Add(sums[0], sums[1])), t = Split(Add(slopes[0], slopes[1]));
-  const float2 both = WarpSum2F(s.x + s.y, t.x + t.y);
-  if (lane == 0) {
-    sh.high[warp] = warp_high;
-    sh.sums[warp] = both;
-  }
-  if (kTop) {
-    sh.group[tid] = group[0];
-    sh.group[kTeam + tid] = group[1];
+// The places of a row's keys where the blocks of a cluster have been through a slice each: every
+// block finds those of its own.
+__device__ __forceinline__ void PlaceTogether(const TokenOut &out, TokenTogether &together,
+                                              int32_t top_k, int32_t r, uint32_t cluster,
+                                              uint32_t rank, int32_t tid, int32_t team, float high,
+                                              float sum) {
+  const float log_sum = logf(sum);
+  int32_t others = 0;
+  for (uint32_t b = 0; b < cluster; ++b) {
+    if (b == rank) continue;
+    const int32_t n = ReadFrom(&together.top, b);
+    for (int32_t k = tid; k < n; k += team)
+      together.others[others + k] = ReadFrom(&together.list[k], b);
+    others += n;
   }
   __syncthreads();
-  float high = sh.high[0];
-#pragma unroll
-  for (int w = 1; w < kTeam / 32; ++w) high = fmaxf(high, sh.high[w]);
-  const float from = high == -INFINITY ? 0.0f : high;
-  float sum = 0.0f, slope = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kTeam / 32; ++w)
-    Join(sum, slope, sh.sums[w].x, sh.sums[w].y, sh.high[w] - from);
-
-  int32_t found = 0;
-  const int32_t top_k = max(0, min(out.top_k, min(span.classes, span.Column(last)) -
-                                                 max(0, span.Column(first))));
-  if (kTop) {
-    // the bound of the top classes
-    if (warp == 0) {
-      constexpr int kAll = 2 * kTeam / 32;
-      uint32_t order[kAll], bound;
-#pragma unroll
-      for (int g = 0; g < kAll; ++g) order[g] = OrderOf(sh.group[32 * g + lane]);
-      if (top_k <= 32) {
-        uint32_t two[2] = {0, 0};
-#pragma unroll
-        for (int g = 0; g < kAll; ++g) two[g & 1] = max(two[g & 1], order[g]);
-        const uint32_t one[1] = {max(two[0], two[1])};
-        bound = top_k <= 16 ? BoundOf(one, top_k) : BoundOf(two, top_k);
-      } else {
-        bound = BoundOf(order, top_k);
+  for (int32_t k = tid; k < top_k; k += team) {
+    const uint64_t key = together.list[k];
+    int32_t place = k, begin = 0;
+    for (uint32_t b = 0; b < cluster; ++b) {
+      if (b == rank) continue;
+      // how many of a list that falls are larger
+      const int32_t n = ReadFrom(&together.top, b);
+      int32_t low = 0, far = n;
+      while (low < far) {
+        const int32_t mid = (low + far) / 2;
+        if (together.others[begin + mid] > key) low = mid + 1; else far = mid;
       }
-      if (lane == 0) {
-        sh.bound = bound;
-        sh.found = 0;
-      }
+      place += low;
+      begin += n;
     }
-    __syncthreads();
-    const float least = ScoreOf(sh.bound);
-    const auto collect = [&](int32_t tile) {
-      const Below<T, kVectors> below(v, span.row, least);
-#pragma unroll
-      for (int w = 0; w < below.kWords; ++w) {
-        uint32_t hits = below.Not(w);
-        while (hits) {
-          const int32_t bit = __clz(hits), k = 32 * w + bit;
-          hits &= ~(0x80000000u >> bit);
-          const int32_t j = tile + k / kPer<T> * kTeam + tid, c = span.Column(j) + k % kPer<T>;
-          if (j >= last || c < 0 || c >= span.classes) continue;
-          const int32_t place = atomicAdd(&sh.found, 1);
-          if (place < out.room) keys[place] = KeyOf(ToFloat(span.row[c]), c);
-        }
-      }
-    };
-    if constexpr (kAgain) {
-      for (int32_t tile = first; tile < last; tile += kTeam * kVectors) {
-        LoadTile<kTeam, kVectors>(v, span, rows, tile, last, tid);
-        collect(tile);
-      }
-    } else {
-      collect(first);
-    }
-    __syncthreads();
-    found = sh.found;
-    if (found > out.room) {
-      const uint64_t bound = RaiseBound(
-          (uint64_t)sh.bound << 32, top_k, out.room, span.classes, [&](uint64_t key) {
-            int32_t n = 0;
-            EachKey<kTeam>(span, first, last, tid, key, [&](uint64_t) { ++n; });
-            n = __reduce_add_sync(0xffffffffu, n);
-            __syncthreads();
-            if (lane == 0) sh.counted[warp] = n;
-            __syncthreads();
-            n = 0;
-#pragma unroll
-            for (int w = 0; w < kTeam / 32; ++w) n += sh.counted[w];
-            return n;
-          });
-      __syncthreads();
-      if (tid == 0) sh.found = 0;
-      __syncthreads();
-      EachKey<kTeam>(span, first, last, tid, bound,
-                     [&](uint64_t key) { keys[atomicAdd(&sh.found, 1)] = key; });
-      __syncthreads();
-      found = sh.found;
-    }
+    if (place < out.top_k) WriteTop(out, r, place, key, high, sum, log_sum);
   }
+}
 
-  if constexpr (kTeam == 256) {
-    if (cluster > 1) {
-      // the first block of a cluster has the row's sums; each finds the places of its own keys
-      if (kTop)
-        for (int32_t k = tid; k < found; k += kTeam) {
-          const uint64_t key = keys[k];
-          int32_t place = 0;
-          for (int32_t o = 0; o < found; ++o) place += keys[o] > key;
-          if (place < top_k) together.list[place] = key;
+// Longer rows: a warp (kTeam 32, several to a block) or a block is a team, or a cluster of blocks
+// (kTeam 512), to which a row's vectors are dealt out in slices.  Rows come 32 at a time, as in
+// TokenWarps; the first warp of a row's first block computes what the rows have one of.  tiles > 1: a
+// slice does not fit, and is read again, part by part, for each pass.
+template <typename T, int kTeam, bool kTop>
+__global__ void
+__launch_bounds__(kTeam == 32 ? 128 : kTeam, kTeam <= 128 ? 6 : kTeam == 256 ? 3 : 2)
+TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
+  extern __shared__ uint4 shared[];
+  __shared__ TokenShared<kTeam> all_shared[kTeam == 32 ? 4 : 1];
+  __shared__ typename std::conditional<kTop && kTeam == 512, TokenTogether, int32_t>::type together;
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31,
+                teams = kTeam == 32 ? (int32_t)blockDim.x / 32 : 1,
+                team = kTeam == 32 ? warp : 0,
+                tid = kTeam == 32 ? lane : (int32_t)threadIdx.x;
+  const uint32_t cluster = kTeam == 512 ? ClusterSize() : 1,
+                 rank = kTeam == 512 ? ClusterRank() : 0;
+  TokenShared<kTeam> &sh = all_shared[team];
+  const int32_t stage = kTeam * vectors;
+  uint4 *slot = shared + team * stage + tid;
+  uint64_t *keys = reinterpret_cast<uint64_t *>(shared + teams * stage) + team * out.room;
+  const int32_t apart = (int32_t)(gridDim.x / cluster) * teams;
+  const bool slopes = out.entropy || out.norm,
+             speaks = rank == 0 && (kTeam == 32 || warp == 0);
+  int32_t parity = 0;
+  for (int32_t base = (int32_t)(blockIdx.x / cluster) * teams + team; base < rows.count;
+       base += 32 * apart) {
+    const int32_t mine = base + lane * apart,
+                  taken = min(32, (rows.count - base + apart - 1) / apart);
+    const T *my_row = nullptr;
+    int64_t token = -1;
+    float score = 0.0f, my_high = 0.0f, my_sum = 0.0f, my_slope = 0.0f;
+    if (lane < taken) {
+      const RowPlace at = PlaceOf(rows, mine);
+      if (at.counts) {
+        my_row = rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride;
+        if (out.log_probs && speaks) {
+          token = IntAt(out.tokens, out.tokens_64, mine);
+          if (token >= 0 && token < rows.classes) score = ToFloat(my_row[token]);
         }
-      if (tid == 0) {
-        together.high = high;
-        together.sum = sum;
-        together.slope = slope;
-        together.top = kTop ? top_k : 0;
       }
-      ClusterSync();
-      for (uint32_t b = 0; b < cluster; ++b) high = fmaxf(high, ReadFrom(&together.high, b));
-      const float all_from = high == -INFINITY ? 0.0f : high;
-      sum = slope = 0.0f;
-      for (uint32_t b = 0; b < cluster; ++b)
-        Join(sum, slope, ReadFrom(&together.sum, b), ReadFrom(&together.slope, b),
-             ReadFrom(&together.high, b) - all_from);
-      if (tid == 0 && rank == 0)
-        Finish(out, r, rows.classes, token, token_score, all_from, sum, slope);
-      if (kTop) {
-        const float log_sum = logf(sum);
-        int32_t others = 0;
-        for (uint32_t b = 0; b < cluster; ++b) {
-          if (b == rank) continue;
-          const int32_t n = ReadFrom(&together.top, b);
-          for (int32_t k = tid; k < n; k += kTeam)
-            together.others[others + k] = ReadFrom(&together.list[k], b);
-          others += n;
+    }
+    const auto row_of = [&](int32_t q) {
+      return reinterpret_cast<const T *>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(my_row), q & 31));
+    };
+    // this thread's part of this block's slice of a row
+    const auto part_of = [&](const T *row) {
+      const RowSpan<T> span(row, rows.classes);
+      const int32_t slice = (span.vectors + (int32_t)cluster - 1) / (int32_t)cluster;
+      const int32_t first = min(span.vectors, (int32_t)rank * slice),
+                    last = min(span.vectors, first + slice);
+      return RowPart<T>(span, first, last, tid, kTeam);
+    };
+    const T *next = row_of(0);
+    if (tiles == 1 && next != nullptr) SendFor<kTeam, 0>(slot, part_of(next), rows);
+    for (int32_t q = 0; q < taken; ++q) {
+      const int32_t r = base + q * apart;
+      const T *row = next;
+      next = q + 1 < taken ? row_of(q + 1) : nullptr;
+      const RowPart<T> whole = part_of(row), coming = part_of(next);
+      const RowPart<T> *const then = tiles == 1 && next != nullptr ? &coming : nullptr;
+      if (row == nullptr) {
+        if (kTop && rank == 0) SkipTop(out, r, tid, kTeam);
+        if (then) SendFor<kTeam, 0>(slot, coming, rows);
+        continue;  // (all blocks of the cluster)
+      }
+      WaitForAll();
+      const Refill<kTeam, T> refill(then, rows);
+      const RowSpan<T> &span = whole.span;
+      const int32_t first = whole.first - tid, last = whole.last;
+      // f(part) for each part of the slice, which is there
+      const auto each = [&](auto &&f) {
+        if (tiles == 1) {
+          f(whole);
+          return;
+        }
+        for (int32_t tile = first; tile < last; tile += stage) {
+          const RowPart<T> part(span, tile, min(last, tile + stage), tid, kTeam);
+          SendFor<kTeam, 0>(slot, part, rows);
+          WaitForAll();
+          f(part);
+        }
+      };
+      // the largest score, of the warp and of four groups of each thread's; the warp's sums
+      Sums sums = NoSums();
+      each([&](const RowPart<T> &part) {
+        CutEnds<kTeam>(slot, part);
+        if constexpr (kTop) {
+          if (slopes)
+            AddRow<true, kTeam>(sums, slot, part.mine, row, kLog2e, NoRefill());
+          else
+            AddRow<false, kTeam>(sums, slot, part.mine, row, kLog2e, NoRefill());
+        } else {
+          if (slopes)
+            AddRow<true, kTeam>(sums, slot, part.mine, row, kLog2e, refill);
+          else
+            AddRow<false, kTeam>(sums, slot, part.mine, row, kLog2e, refill);
+        }
+      });
+      if (!kTop) refill.Rest(slot, whole.mine, then, rows);
+      float high;
+      float2 both = slopes ? WarpSums<true>(sums, kLog2e, &high)
+                           : WarpSums<false>(sums, kLog2e, &high);
+      if (kTeam > 32) {
+        // (a warp is at most one barrier ahead: the values of the row before are still read)
+        parity ^= 1;
+        if (lane == 0) {
+          sh.high[parity][warp] = high;
+          sh.sums[parity][warp] = both;
+        }
+        if (kTop) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) sh.group[g * kTeam + tid] = sums.group[g];
         }
         __syncthreads();
-        for (int32_t k = tid; k < top_k; k += kTeam) {
-          const uint64_t key = together.list[k];
-          int32_t place = k, begin = 0;
-          for (uint32_t b = 0; b < cluster; ++b) {
-            if (b == rank) continue;
-            // how many of a list that falls are larger
-            const int32_t n = ReadFrom(&together.top, b);
-            int32_t low = 0, far = n;
-            while (low < far) {
-              const int32_t mid = (low + far) / 2;
-              if (together.others[begin + mid] > key) low = mid + 1; else far = mid;
-            }
-            place += low;
-            begin += n;
-          }
-          if (place < out.top_k) WriteTop(out, r, place, key, all_from, sum, log_sum);
+        // (without top classes or a cluster nobody else needs them)
+        if (kTop || cluster > 1 || warp == 0) {
+          const bool one = lane < kTeam / 32;
+          const float h = one ? sh.high[parity][lane] : -INFINITY;
+          const float2 part = one ? sh.sums[parity][lane] : make_float2(0.0f, 0.0f);
+          both = JoinWarp(h, part, &high);
         }
       }
-      ClusterSync();  // nobody leaves while others read its memory
-      return;
+      int32_t found = 0;
+      const int32_t top_k = max(0, min(out.top_k, min(span.classes, span.Column(last)) -
+                                                     max(0, span.Column(first))));
+      if (kTop) {
+        // the bound of the top classes
+        if (kTeam == 32 || warp == 0) {
+          uint32_t bound, four[4];
+          if (kTeam == 32) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) four[g] = OrderOf(sums.group[g]);
+          } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) four[g] = 0;
+#pragma unroll 4
+            for (int g = 0; g < 4 * kTeam / 32; g += 4)
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                four[u] = max(four[u], OrderOf(sh.group[32 * (g + u) + lane]));
+          }
+          if (top_k <= 16) {
+            const uint32_t one[1] = {max(max(four[0], four[1]), max(four[2], four[3]))};
+            bound = BoundOf(one, top_k);
+          } else {
+            bound = BoundOf(four, top_k);
+          }
+          if (lane == 0) {
+            sh.bound = bound;
+            sh.found = 0;
+          }
+        }
+        TeamSync<kTeam>();
+        const float least = ScoreOf(sh.bound);
+        each([&](const RowPart<T> &part) {
+          if (tiles > 1) CutEnds<kTeam>(slot, part);
+          CollectRow<kTeam>(slot, part, least, keys, out.room, &sh.found, refill);
+        });
+        refill.Rest(slot, whole.mine, then, rows);
+        TeamSync<kTeam>();
+        found = sh.found;
+        if (found > out.room) {
+          const uint64_t bound = RaiseBound(
+              (uint64_t)sh.bound << 32, top_k, out.room, span.classes, [&](uint64_t key) {
+                int32_t n = 0;
+                EachKey<kTeam>(span, first, last, tid, key, [&](uint64_t) { ++n; });
+                n = __reduce_add_sync(0xffffffffu, n);
+                if (kTeam > 32) {
+                  __syncthreads();
+                  if (lane == 0) sh.counted[warp] = n;
+                  __syncthreads();
+                  n = 0;
+#pragma unroll
+                  for (int w = 0; w < kTeam / 32; ++w) n += sh.counted[w];
+                }
+                return n;
+              });
+          TeamSync<kTeam>();
+          if (tid == 0) sh.found = 0;
+          TeamSync<kTeam>();
+          EachKey<kTeam>(span, first, last, tid, bound,
+                         [&](uint64_t key) { keys[Count(&sh.found)] = key; });
+          TeamSync<kTeam>();
+          found = sh.found;
+        }
+      }
+      if (kTeam == 512 && cluster > 1) {
+        if constexpr (kTop && kTeam == 512) {
+          EachPlace(keys, found, tid, kTeam, [&](int32_t at, uint64_t key) {
+            if (at < top_k) together.list[at] = key;
+          });
+          if (tid == 0) together.top = top_k;
+        }
+        if (tid == 0) {
+          sh.all_high = high;
+          sh.all_sums = both;
+        }
+        ClusterSync();
+        const bool one = lane < (int32_t)cluster;
+        const float h = one ? ReadFrom(&sh.all_high, lane) : -INFINITY;
+        const float2 part = one ? ReadFrom(&sh.all_sums, lane) : make_float2(0.0f, 0.0f);
+        both = JoinWarp(h, part, &high);
+        if constexpr (kTop && kTeam == 512)
+          PlaceTogether(out, together, top_k, r, cluster, rank, tid, kTeam,
+                        high == -INFINITY ? 0.0f : high, both.x);
+        ClusterSync();  // nobody goes on while others read its memory
+      } else if (kTop) {
+        const float log_sum = logf(both.x), from = high == -INFINITY ? 0.0f : high;
+        EachPlace(keys, found, tid, kTeam, [&](int32_t at, uint64_t key) {
+          if (at < out.top_k) WriteTop(out, r, at, key, from, both.x, log_sum);
+        });
+        // (the next row's keys come to the same place, in a block behind two more barriers)
+        if (kTeam == 32) __syncwarp();
+      }
+      if (lane == q) {
+        my_high = high == -INFINITY ? 0.0f : high;
+        my_sum = both.x;
+        my_slope = both.y;
+      }
     }
-  }
-  if (tid == 0) Finish(out, r, rows.classes, token, token_score, from, sum, slope);
-  if (kTop) {
-    const float log_sum = logf(sum);
-    for (int32_t k = tid; k < found; k += kTeam) {
-      const uint64_t key = keys[k];
-      int32_t place = 0;
-      for (int32_t o = 0; o < found; ++o) place += keys[o] > key;
-      if (place < out.top_k) WriteTop(out, r, place, key, from, sum, log_sum);
+    if (speaks && lane < taken) {
+      if (my_row != nullptr)
+        Finish(out, mine, rows.classes, token, score, my_high, my_sum, my_slope);
+      else
+        SkipRow(out, mine);
     }
   }
 }
@@ -573,17 +659,36 @@ __device__ __forceinline__ float GradAt(const k2b200_row_grad &g, RowPlace at, i
 }
 
 // dL/dx_c = -p_c (all + slope * (log p_c + h)), with `all` the upstream of every log-prob of the
-// row; what a class gets as a given or a top one is added where it is.
+// row; what a class gets as a given or a top one is added where it is.  As 2^((x - high) log2 e) *
+// (constant + by * (x - high)); the clamp leaves 0 and not 0 * -inf where p is 0.
 struct Spread {
-  float high, inverse, all, slope, offset;
+  float high, constant, by;
   __device__ __forceinline__ float operator()(float x) const {
-    const float d = x - high, p = Exp2(d * kLog2e) * inverse;
-    return p == 0.0f ? 0.0f : -p * fmaf(slope, d + offset, all);
+    const float d = x - high;
+    return Exp2(d * kLog2e) * (by == 0.0f ? constant : fmaf(by, fmaxf(d, -200.0f), constant));
+  }
+  template <typename T>
+  __device__ __forceinline__ void operator()(const uint4 &v, const T *type,
+                                             float (&f)[kPer<T>]) const {
+    const Two minus = MakeTwo(-high, -high), k = MakeTwo(kLog2e, kLog2e),
+              c = MakeTwo(constant, constant), b = MakeTwo(by, by);
+    EachPair(v, type, [&](float2 x, int pair) {
+      const Two d = Add(MakeTwo(x.x, x.y), minus);
+      const float2 t = Split(Mul(d, k)), s = Split(d);
+      const Two e = MakeTwo(Exp2(t.x), Exp2(t.y));
+      const float2 g =
+          Split(by == 0.0f
+                    ? Mul(e, c)
+                    : Mul(e, Fma(b, MakeTwo(fmaxf(s.x, -200.0f), fmaxf(s.y, -200.0f)), c)));
+      f[2 * pair] = g.x;
+      f[2 * pair + 1] = g.y;
+    });
   }
 };
 
-// A team per row and kTile vectors per thread of it at a time: the norm is known, so every class
-// is on its own.  The classes that are a given or a top one are written again behind the others.
+// A team per row, or per part of `part` vectors of one: the norm is known, so every class is on its
+// own.  Four vectors per thread are read while the four before them are worked on.  The classes that
+// are a given or a top one are written again behind the others.
 template <typename T, int kTeam, bool kTop>
 __global__ void __launch_bounds__(256, 4)
 TokenScoresBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t part) {
@@ -593,23 +698,28 @@ TokenScoresBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t p
   const int32_t r = kTeam == 32 ? (int32_t)(blockIdx.x * (blockDim.x >> 5)) + warp
                                 : (int32_t)(blockIdx.x / (uint32_t)parts);
   if (r >= rows.count) return;
-  const int32_t slice = kTeam == 32 ? 0 : (int32_t)(blockIdx.x % (uint32_t)parts);
+  const int32_t first = kTeam == 32 ? 0 : (int32_t)(blockIdx.x % (uint32_t)parts) * part;
   const RowPlace at = PlaceOf(rows, r);
   T *out = grad + at.o * g.outer_stride + at.i * g.inner_stride;
   if (!at.counts) {
-    const RowSpan<T> zeros(out, rows.classes);
-    const float f[kPer<T>] = {};
-    const int32_t end = kTeam == 32 ? zeros.vectors : min(zeros.vectors, (slice + 1) * part);
-    for (int32_t j = slice * part + tid; j < end; j += kTeam) Store(out, zeros, true, j, f);
+    WriteZeros(out, rows.classes, first, kTeam == 32 ? INT32_MAX : first + part, tid, kTeam);
     return;
   }
   const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
                         rows.classes);
   const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
-  const int32_t first = slice * part,
-                last = kTeam == 32 ? span.vectors : min(span.vectors, first + part);
+  const int32_t last = kTeam == 32 ? span.vectors : min(span.vectors, first + part);
+  // vectors [from, to) are whole
+  const int32_t from = first < last && !span.Whole(span.Column(first)) ? first + 1 : first,
+                to = last > from && !span.Whole(span.Column(last - 1)) ? last - 1 : last;
+  const uint4 *in = reinterpret_cast<const uint4 *>(span.row - span.shift);
   uint4 v[kTile];
-  LoadTile<kTeam, kTile>(v, span, rows, first, last, tid);
+  const auto load = [&](int32_t tile) {
+#pragma unroll
+    for (int i = 0; i < kTile; ++i)
+      if (tile + i * kTeam < to) v[i] = in[tile + i * kTeam];
+  };
+  load(from + tid);
   const float4 n = g.norm[r];
   const int64_t token = g.log_probs.grad ? IntAt(g.tokens, g.tokens_64, r) : -1;
   const bool some = token >= 0 && token < rows.classes;
@@ -620,24 +730,39 @@ TokenScoresBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t p
     for (int32_t k = lane; k < g.top_k; k += 32) top_sum += GradAt(g.top, at, k);
     top_sum = WarpSumF(top_sum);
   }
+  const float slope = GradAt(g.entropy, at), inverse = n.y == 0.0f ? 0.0f : 1.0f / n.y;
   Spread spread;
   spread.high = n.x;
-  spread.inverse = n.y == 0.0f ? 0.0f : 1.0f / n.y;
-  spread.all = token_grad + top_sum;
-  spread.slope = GradAt(g.entropy, at);
-  spread.offset = n.z - logf(n.y);
-  for (int32_t tile = first; tile < last; tile += kTeam * kTile) {
-    if (tile != first) LoadTile<kTeam, kTile>(v, span, rows, tile, last, tid);
+  spread.by = -slope * inverse;
+  // (a row without a class left: no class has a share)
+  spread.constant =
+      n.y == 0.0f ? 0.0f : -inverse * fmaf(slope, n.z - logf(n.y), token_grad + top_sum);
+  const auto store = [&](int32_t j, const uint4 &x, bool whole) {
+    float f[kPer<T>];
+    spread(x, span.row, f);
+    if (whole && aligned)
+      *reinterpret_cast<uint4 *>(out + span.Column(j)) = Pack(f, out);
+    else
+      Store(out, span, false, j, f);
+  };
+  for (int32_t tile = from + tid; tile < to; tile += kTeam * kTile) {
+    uint4 x[kTile];
 #pragma unroll
-    for (int i = 0; i < kTile; ++i) {
-      const int32_t j = tile + i * kTeam + tid;
-      if (j >= last) continue;
-      float f[kPer<T>];
-      Unpack(Packed(v[i]), f, span.row);
+    for (int i = 0; i < kTile; ++i) x[i] = v[i];
+    load(tile + kTeam * kTile);
+    if (aligned) {
 #pragma unroll
-      for (int k = 0; k < kPer<T>; ++k) f[k] = spread(f[k]);
-      Store(out, span, aligned, j, f);
+      for (int i = 0; i < kTile; ++i)
+        if (tile + i * kTeam < to) store(tile + i * kTeam, x[i], true);
+    } else {
+#pragma unroll 1
+      for (int32_t j = tile; j < min(to, tile + kTeam * kTile); j += kTeam) store(j, in[j], false);
     }
+  }
+  // the row's ends
+  if (tid < 2) {
+    const int32_t j = tid == 0 ? first : last - 1;
+    if ((j < from || j >= to) && j < last && (tid == 0 || j > first)) store(j, span.Edge(j), false);
   }
   // behind the stores of the other threads: the token, unless a top class, and the top classes
   TeamSync<kTeam>();
@@ -672,23 +797,22 @@ namespace {
 template <typename T, bool kTop>
 int32_t LaunchTokenScores(const k2b200_class_rows *rows, const TokenOut &out, cudaStream_t s) {
   const Rows<T> r = RowsOf<T>(rows);
-  const RowPlan p = PlanRows(r);
-  if (p.team == 32) {
+  const int32_t key_bytes = (int32_t)sizeof(uint64_t) * out.room;
+  const RowPlan p = PlanRows(r, key_bytes);
+  const size_t smem = (size_t)p.ring + (size_t)key_bytes * (p.block / p.team);
+  if (p.in_registers) {
     auto kernel = p.vectors == 1   ? TokenWarps<T, 1, kTop>
                   : p.vectors == 2 ? TokenWarps<T, 2, kTop>
                   : p.vectors == 4 ? TokenWarps<T, 4, kTop>
                                    : TokenWarps<T, 8, kTop>;
-    kernel<<<CeilDiv(r.count, p.rows_per_block), p.block,
-             sizeof(uint64_t) * out.room * (p.block / 32), s>>>(r, out, p.rows_per_warp);
+    kernel<<<(uint32_t)p.blocks, p.block, smem, s>>>(r, out);
   } else {
-    auto kernel = p.team == 128   ? (p.vectors == 4 ? TokenBlocks<T, 128, 4, kTop, false>
-                                                    : TokenBlocks<T, 128, 8, kTop, false>)
-                  : p.again        ? TokenBlocks<T, 256, 16, kTop, true>
-                  : p.vectors == 4 ? TokenBlocks<T, 256, 4, kTop, false>
-                  : p.vectors == 8 ? TokenBlocks<T, 256, 8, kTop, false>
-                                   : TokenBlocks<T, 256, 16, kTop, false>;
-    K2B_CUDA_OK(LaunchRows(kernel, (int64_t)r.count * p.cluster, p.block,
-                           sizeof(uint64_t) * out.room, p.cluster, false, s, r, out));
+    auto kernel = p.team == 32    ? TokenRing<T, 32, kTop>
+                  : p.team == 256 ? TokenRing<T, 256, kTop>
+                                  : TokenRing<T, 512, kTop>;
+    K2B_CUDA_OK(AllowShared(kernel, smem));
+    K2B_CUDA_OK(LaunchRows(kernel, p.blocks, p.block, smem, p.cluster, false, s, r, out, p.vectors,
+                           p.tiles));
   }
   NoteLaunch();
   K2B_CUDA_OK(cudaGetLastError());
@@ -699,19 +823,22 @@ template <typename T>
 int32_t LaunchTokenBackward(const k2b200_class_rows *rows, const TokenGrad &g, void *grad,
                             cudaStream_t s) {
   const Rows<T> r = RowsOf<T>(rows);
-  const RowPlan p = PlanRows(r);
   T *out = static_cast<T *>(grad);
   const bool top = g.top_k > 0;
-  // vectors of a row, wherever it begins, in parts of 1024: a block's four per thread
-  const int32_t vectors =
-      (int32_t)((rows->num_classes + kPer<T> - 1) / kPer<T>) + (kPer<T> > 1 ? 1 : 0);
-  if (p.team == 32) {
+  // vectors of a row, wherever it begins: up to 256 of them are a warp's; more are dealt out to
+  // blocks in parts of 4096, 16 per thread, or of 1024 where that is too few blocks (4096 x 32001
+  // bf16: 102 us in parts of 1024, 83 of 2048, 77 of 4096, at the memory's rate)
+  const int32_t vectors = CeilDiv((int64_t)r.classes + kPer<T> - 1, kPer<T>) + 1;
+  if (vectors <= 256) {
+    const int32_t warps =
+        (int32_t)std::min<int64_t>(8, std::max<int64_t>(1, r.count / NumSms()));
     auto kernel = top ? TokenScoresBackward<T, 32, true> : TokenScoresBackward<T, 32, false>;
-    kernel<<<CeilDiv(r.count, p.block / 32), p.block, 0, s>>>(r, g, out, 1, 0);
+    kernel<<<CeilDiv(r.count, warps), 32 * warps, 0, s>>>(r, g, out, 1, 0);
   } else {
-    const int32_t part = 1024, parts = CeilDiv(vectors, part);
+    const int32_t part = CeilDiv(vectors, 4096) * (int64_t)r.count >= 2 * NumSms() ? 4096 : 1024,
+                  parts = CeilDiv(vectors, part);
     K2B_REQUIRE((int64_t)parts * r.count < ((int64_t)1 << 31), "too many rows of %d classes",
-                rows->num_classes);
+                r.classes);
     auto kernel = top ? TokenScoresBackward<T, 256, true> : TokenScoresBackward<T, 256, false>;
     kernel<<<(uint32_t)((int64_t)parts * r.count), 256, 0, s>>>(r, g, out, parts, part);
   }
