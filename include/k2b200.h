@@ -888,7 +888,8 @@ typedef struct {
  * and p = softmax(x / T) over all classes.  A row without an entry of finite score gives 0.
  * loss: [rows], or one value.  grad_scores (may be NULL): the gradient of the sum or mean,
  * as in k2b200_token_scores_backward.  norm [rows, 4] (NULL: no backward pass follows).
- * workspace: k2b200_distillation_workspace_bytes(); the backward pass reads it. */
+ * workspace: k2b200_distillation_workspace_bytes(), none without a reduction; the backward pass
+ * reads it. */
 size_t k2b200_distillation_workspace_bytes(const k2b200_class_rows *rows);
 int32_t k2b200_distillation(const k2b200_class_rows *rows, const k2b200_teacher *teacher,
                             float *loss, float *norm, void *grad_scores,

@@ -797,7 +797,8 @@ int32_t LaunchDistil(const k2b200_class_rows *rows, const k2b200_teacher *t, flo
   const Teacher teacher = {t->tokens, t->scores, t->tokens_64, t->type, t->entries,
                            t->temperature};
   const DistilBy by = ByOf(rows, t, workspace);
-  double *partial = reinterpret_cast<double *>(static_cast<char *>(workspace) + kDistilHead);
+  double *partial =
+      workspace ? reinterpret_cast<double *>(static_cast<char *>(workspace) + kDistilHead) : nullptr;
   if (by.device) {
     DistilCount<<<1, 1024, 0, s>>>(rows->lengths, rows->lengths_64, rows->outer, rows->inner,
                                    t->weight, static_cast<DistilScale *>(workspace));
@@ -869,7 +870,10 @@ int32_t LaunchDistilBackward(const k2b200_class_rows *rows, const k2b200_teacher
 extern "C" {
 
 size_t k2b200_distillation_workspace_bytes(const k2b200_class_rows *rows) {
-  return rows ? kDistilHead + sizeof(double) * (size_t)(rows->outer * rows->inner) : 0;
+  if (rows == nullptr) return 0;
+  // (a loss per block: PlanRows has at most 64 of them on an SM)
+  return kDistilHead + sizeof(double) * (size_t)std::min<int64_t>(rows->outer * rows->inner,
+                                                                  64 * (int64_t)NumSms());
 }
 
 int32_t k2b200_distillation(const k2b200_class_rows *rows, const k2b200_teacher *teacher,
@@ -880,12 +884,13 @@ int32_t k2b200_distillation(const k2b200_class_rows *rows, const k2b200_teacher 
   K2B_FORWARD(CheckTeacher(teacher, rows));
   K2B_REQUIRE(!grad_scores || teacher->reduction != 0,
               "the gradient of row losses needs their upstream");
-  K2B_REQUIRE(workspace, "NULL pointer");
+  const size_t need =
+      teacher->reduction == 0 ? 0 : k2b200_distillation_workspace_bytes(rows);
+  K2B_REQUIRE(workspace || need == 0, "NULL pointer");
   K2B_REQUIRE(loss || (teacher->reduction == 0 && rows->outer * rows->inner == 0),
               "NULL pointer");
-  if (workspace_bytes < k2b200_distillation_workspace_bytes(rows)) {
-    SetError("workspace of %zu bytes, %zu are needed", workspace_bytes,
-             k2b200_distillation_workspace_bytes(rows));
+  if (workspace_bytes < need) {
+    SetError("workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     return kWorkspaceTooSmall;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -905,9 +910,11 @@ int32_t k2b200_distillation_backward(const k2b200_class_rows *rows, const k2b200
   K2B_FORWARD(CheckRows(rows));
   K2B_FORWARD(CheckTeacher(teacher, rows));
   if (rows->outer * rows->inner == 0) return kOk;
-  K2B_REQUIRE(norm && upstream && upstream->grad && grad_scores && workspace, "NULL pointer");
-  if (workspace_bytes < kDistilHead) {
-    SetError("workspace of %zu bytes, %zu are needed", workspace_bytes, kDistilHead);
+  const size_t need = teacher->reduction == 0 ? 0 : kDistilHead;
+  K2B_REQUIRE(norm && upstream && upstream->grad && grad_scores && (workspace || need == 0),
+              "NULL pointer");
+  if (workspace_bytes < need) {
+    SetError("workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     return kWorkspaceTooSmall;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
