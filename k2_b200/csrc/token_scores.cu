@@ -59,6 +59,54 @@ __device__ __forceinline__ uint32_t BoundOf(const uint32_t (&order)[kGroups], in
   return low;
 }
 
+// The keys that a team collects: score and class in one number (OrderOf), which sorts as they do.
+// A warp's rows have at most 8192 classes, so that with a score of 16 bits a key is one of 32.
+template <typename T, int kTeam>
+struct Keys {
+  using Key = uint64_t;
+  __device__ __forceinline__ static Key Make(T x, int32_t c) { return KeyOf(ToFloat(x), c); }
+  __device__ __forceinline__ static Key From(uint64_t key) { return key; }
+  __device__ __forceinline__ static float Score(Key key) { return ScoreOf((uint32_t)(key >> 32)); }
+  __device__ __forceinline__ static int32_t Class(Key key) { return (int32_t)~(uint32_t)key; }
+};
+struct ShortKeys {
+  using Key = uint32_t;
+  __device__ __forceinline__ static Key Make(uint32_t bits, uint32_t infinity, int32_t c) {
+    uint32_t order = bits & 0x8000u ? ~bits & 0xffffu : bits | 0x8000u;
+    if (bits == 0x8000u) order = 0x8000u;              // -0 is 0
+    if ((bits & 0x7fffu) > infinity) order = 0xffffu;  // NaN
+    return order << 16 | (~(uint32_t)c & 0xffffu);
+  }
+  __device__ __forceinline__ static uint16_t Bits(Key key) {
+    return (uint16_t)(key & 0x80000000u ? key >> 16 & 0x7fffu : ~(key >> 16));
+  }
+  __device__ __forceinline__ static int32_t Class(Key key) { return (int32_t)(~key & 0xffffu); }
+};
+template <>
+struct Keys<__half, 32> : ShortKeys {
+  __device__ __forceinline__ static Key Make(__half x, int32_t c) {
+    return ShortKeys::Make(__half_as_ushort(x), 0x7c00u, c);
+  }
+  __device__ __forceinline__ static Key From(uint64_t key) {
+    return Make(__float2half_rn(ScoreOf((uint32_t)(key >> 32))), (int32_t)~(uint32_t)key);
+  }
+  __device__ __forceinline__ static float Score(Key key) {
+    return __half2float(__ushort_as_half(Bits(key)));
+  }
+};
+template <>
+struct Keys<__nv_bfloat16, 32> : ShortKeys {
+  __device__ __forceinline__ static Key Make(__nv_bfloat16 x, int32_t c) {
+    return ShortKeys::Make(__bfloat16_as_ushort(x), 0x7f80u, c);
+  }
+  __device__ __forceinline__ static Key From(uint64_t key) {
+    return Make(__float2bfloat16_rn(ScoreOf((uint32_t)(key >> 32))), (int32_t)~(uint32_t)key);
+  }
+  __device__ __forceinline__ static float Score(Key key) {
+    return __uint_as_float((uint32_t)Bits(key) << 16);
+  }
+};
+
 // Bit e is set where score e of a vector is not below `least` (NaN is not).
 __device__ __forceinline__ uint32_t Reaching(const uint4 &v, float least, const float *) {
   return (!(__uint_as_float(v.x) < least) ? 1u : 0u) | (!(__uint_as_float(v.y) < least) ? 2u : 0u) |
@@ -95,11 +143,29 @@ __device__ __forceinline__ int32_t Count(int32_t *found) {
   return at;
 }
 
-// Puts the keys of a thread's scores that reach `least` where there is room, counting them all.  A
-// score's vector is told by its bit, but no register by a number: it is read again, from the cache.
-template <int kTeam, int kVectors, typename T>
-__device__ __forceinline__ void Collect(uint4 (&v)[kVectors], const RowPart<T> &part, float least,
-                                        uint64_t *keys, int32_t room, int32_t *found) {
+// Puts the key of each score whose bit is set, of vectors i0 on, where there is room, and counts them
+// all.
+template <int kTeam, typename T, typename Key>
+__device__ __forceinline__ void PutKeys(uint32_t bits, const uint4 *slot, const RowPart<T> &part,
+                                        int32_t i0, Key *keys, int32_t room, int32_t *found) {
+  while (bits) {
+    const int32_t bit = __ffs(bits) - 1, i = i0 + bit / kPer<T>, e = bit % kPer<T>;
+    bits &= bits - 1;
+    const int32_t c = part.span.Column(part.first + i * kTeam) + e;
+    // (beside the row there is nothing but -inf)
+    if (i >= part.mine || c < 0 || c >= part.span.classes) continue;
+    const int32_t at = Count(found);
+    if (at < room)
+      keys[at] = Keys<T, kTeam>::Make(reinterpret_cast<const T *>(slot + i * kTeam)[e], c);
+  }
+}
+
+// The keys of a thread's scores that reach `least`: of vectors in registers (a score is told by its
+// bit, but no register by a number: it is read from shared memory) ...
+template <int kTeam, int kVectors, typename T, typename Key>
+__device__ __forceinline__ void Collect(uint4 (&v)[kVectors], const uint4 *slot,
+                                        const RowPart<T> &part, float least, Key *keys,
+                                        int32_t room, int32_t *found) {
   constexpr int kWord = 32 / kPer<T>;  // vectors to a word of bits
 #pragma unroll
   for (int i0 = 0; i0 < kVectors; i0 += kWord) {
@@ -107,24 +173,13 @@ __device__ __forceinline__ void Collect(uint4 (&v)[kVectors], const RowPart<T> &
 #pragma unroll
     for (int u = 0; u < kWord && i0 + u < kVectors; ++u)
       bits |= Reaching(Packed(v[i0 + u]), least, part.span.row) << (u * kPer<T>);
-    while (bits) {
-      const int32_t bit = __ffs(bits) - 1;
-      bits &= bits - 1;
-      const int32_t i = i0 + bit / kPer<T>,
-                    c = part.span.Column(part.first + i * kTeam) + bit % kPer<T>;
-      // (beside the row there is nothing but -inf)
-      if (i >= part.mine || c < 0 || c >= part.span.classes) continue;
-      const uint64_t key = KeyOf(ToFloat(part.span.row[c]), c);
-      const int32_t at = Count(found);
-      if (at < room) keys[at] = key;
-    }
+    PutKeys<kTeam>(bits, slot, part, i0, keys, room, found);
   }
 }
-
-// The same for a thread's vectors in shared memory, where a score is read by its number.
-template <int kTeam, typename T, typename F>
+// ... and of vectors in shared memory.
+template <int kTeam, typename T, typename Key, typename F>
 __device__ __forceinline__ void CollectRow(uint4 *slot, const RowPart<T> &part, float least,
-                                           uint64_t *keys, int32_t room, int32_t *found,
+                                           Key *keys, int32_t room, int32_t *found,
                                            const F &then) {
   constexpr int kWord = 32 / kPer<T>;
 #pragma unroll 1
@@ -134,15 +189,7 @@ __device__ __forceinline__ void CollectRow(uint4 *slot, const RowPart<T> &part, 
     for (int u = 0; u < kWord; ++u)
       if (i0 + u < part.mine)
         bits |= Reaching(slot[(i0 + u) * kTeam], least, part.span.row) << (u * kPer<T>);
-    while (bits) {
-      const int32_t bit = __ffs(bits) - 1, i = i0 + bit / kPer<T>, e = bit % kPer<T>;
-      bits &= bits - 1;
-      const int32_t c = part.span.Column(part.first + i * kTeam) + e;
-      // (beside the row there is nothing but -inf)
-      if (c < 0 || c >= part.span.classes) continue;
-      const int32_t at = Count(found);
-      if (at < room) keys[at] = KeyOf(ToFloat(reinterpret_cast<const T *>(slot + i * kTeam)[e]), c);
-    }
+    PutKeys<kTeam>(bits, slot, part, i0, keys, room, found);
 #pragma unroll
     for (int u = 0; u < kWord; ++u)
       if (i0 + u < part.mine) then(slot, i0 + u);
@@ -184,12 +231,13 @@ __device__ __forceinline__ uint64_t RaiseBound(uint64_t bound, int32_t top_k, in
   }
 }
 
+template <typename K>
 __device__ __forceinline__ void WriteTop(const TokenOut &out, int32_t r, int32_t place,
-                                         uint64_t key, float high, float sum, float log_sum) {
+                                         typename K::Key key, float high, float sum,
+                                         float log_sum) {
   const int64_t at = (int64_t)r * out.top_k + place;
-  out.top_tokens[at] = (int32_t)~(uint32_t)key;
-  out.top_log_probs[at] =
-      sum == 0.0f ? -INFINITY : (ScoreOf((uint32_t)(key >> 32)) - high) - log_sum;
+  out.top_tokens[at] = K::Class(key);
+  out.top_log_probs[at] = sum == 0.0f ? -INFINITY : (K::Score(key) - high) - log_sum;
 }
 
 // The values that a row has one of.
@@ -221,17 +269,52 @@ __device__ __forceinline__ void SkipTop(const TokenOut &out, int32_t r, int32_t 
   }
 }
 
-// The places of n keys among them, for those of the top: rank by counting.
-template <typename F>
-__device__ __forceinline__ void EachPlace(const uint64_t *keys, int32_t n, int32_t tid,
-                                          int32_t team, F &&f) {
-  for (int32_t k = tid; k < n; k += team) {
+// f(place, key) for the places of n keys among them, by counting the larger ones: a warp, two keys to
+// a lane at a time.
+template <typename Key, typename F>
+__device__ __forceinline__ void EachPlaceWarp(const Key *keys, int32_t n, int32_t lane, F &&f) {
+  for (int32_t k = lane; k < n; k += 64) {
+    const Key a = keys[k];
+    int32_t place = 0;
+    if (n <= 32) {
+#pragma unroll 4
+      for (int32_t o = 0; o < n; ++o) place += keys[o] > a;
+      f(place, a);
+      continue;
+    }
+    const bool two = k + 32 < n;
+    const Key b = two ? keys[k + 32] : a;
+    int32_t other = 0;
+#pragma unroll 4
+    for (int32_t o = 0; o < n; ++o) {
+      const Key key = keys[o];
+      place += key > a;
+      other += key > b;
+    }
+    f(place, a);
+    if (two) f(other, b);
+  }
+}
+// ... or a block, several threads to a key where there are many (places: room for n numbers).
+template <int kTeam, typename F>
+__device__ __forceinline__ void EachPlaceBlock(const uint64_t *keys, int32_t n, int32_t *places,
+                                               int32_t tid, F &&f) {
+  constexpr int kParts = kTeam / 128;
+  if (n <= 32) {
+    if (tid < 32) EachPlaceWarp(keys, n, tid, f);
+    return;
+  }
+  for (int32_t k = tid; k < n; k += kTeam) places[k] = 0;
+  __syncthreads();
+  for (int32_t k = tid & 127; k < n; k += 128) {
     const uint64_t key = keys[k];
     int32_t place = 0;
 #pragma unroll 4
-    for (int32_t o = 0; o < n; ++o) place += keys[o] > key;
-    f(place, key);
+    for (int32_t o = tid >> 7; o < n; o += kParts) place += keys[o] > key;
+    atomicAdd(&places[k], place);
   }
+  __syncthreads();
+  for (int32_t k = tid; k < n; k += kTeam) f(places[k], keys[k]);
 }
 
 // Short rows: each warp is a team.  It takes 32 rows at a time, a whole grid of warps apart; lane q
@@ -243,8 +326,12 @@ TokenWarps(Rows<T> rows, TokenOut out) {
   extern __shared__ uint4 shared[];
   __shared__ int32_t all_found[4];
   const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  uint4 *slot = shared + warp * 32 * kVectors + lane;
-  uint64_t *keys = reinterpret_cast<uint64_t *>(shared + warps * 32 * kVectors) + warp * out.room;
+  using K = Keys<T, 32>;
+  // (with top classes two rows, since the one at hand is read again)
+  constexpr int32_t kStage = 32 * kVectors, kRows = kTop ? 2 : 1;
+  uint4 *const ring = shared + warp * kRows * kStage + lane;
+  typename K::Key *keys =
+      reinterpret_cast<typename K::Key *>(shared + warps * kRows * kStage) + warp * out.room;
   const int32_t apart = (int32_t)gridDim.x * warps;
   const bool slopes = out.entropy || out.norm;
   for (int32_t base = (int32_t)blockIdx.x * warps + warp; base < rows.count; base += 32 * apart) {
@@ -270,12 +357,14 @@ TokenWarps(Rows<T> rows, TokenOut out) {
     const T *next = row_of(0);
     if (next != nullptr) {
       const RowSpan<T> span(next, rows.classes);
-      SendFor<32, kVectors>(slot, RowPart<T>(span, 0, span.vectors, lane, 32), rows);
+      SendFor<32, kVectors>(ring, RowPart<T>(span, 0, span.vectors, lane, 32), rows);
     }
     for (int32_t q = 0; q < taken; ++q) {
       const T *row = next;
       const RowSpan<T> span(row, rows.classes);
       const RowPart<T> part(span, 0, span.vectors, lane, 32);
+      uint4 *const slot = ring + (kRows > 1 ? q & 1 : 0) * kStage,
+                   *const other = ring + (kRows > 1 ? ~q & 1 : 0) * kStage;
       uint4 v[kVectors];
       if (row != nullptr) {
         WaitForAll();
@@ -285,7 +374,7 @@ TokenWarps(Rows<T> rows, TokenOut out) {
       next = row_of(q + 1);
       if (q + 1 < taken && next != nullptr) {
         const RowSpan<T> coming(next, rows.classes);
-        SendFor<32, kVectors>(slot, RowPart<T>(coming, 0, coming.vectors, lane, 32), rows);
+        SendFor<32, kVectors>(other, RowPart<T>(coming, 0, coming.vectors, lane, 32), rows);
       }
       if (row == nullptr) {
         if (kTop) SkipTop(out, base + q * apart, lane, 32);
@@ -322,7 +411,7 @@ TokenWarps(Rows<T> rows, TokenOut out) {
         }
         if (lane == 0) all_found[warp] = 0;
         __syncwarp();  // (and the keys of the row before have been read)
-        Collect<32>(v, part, least, keys, out.room, &all_found[warp]);
+        Collect<32>(v, slot, part, least, keys, out.room, &all_found[warp]);
         __syncwarp();
         int32_t found = all_found[warp];
         if (found > out.room) {
@@ -337,14 +426,14 @@ TokenWarps(Rows<T> rows, TokenOut out) {
           if (lane == 0) all_found[warp] = 0;
           __syncwarp();
           EachKey<32>(span, 0, span.vectors, lane, bound,
-                      [&](uint64_t key) { keys[atomicAdd(&all_found[warp], 1)] = key; });
+                      [&](uint64_t key) { keys[Count(&all_found[warp])] = K::From(key); });
           __syncwarp();
           found = all_found[warp];
         }
         const float log_sum = logf(sum);
-        EachPlace(keys, found, lane, 32, [&](int32_t place, uint64_t key) {
+        EachPlaceWarp(keys, found, lane, [&](int32_t place, typename K::Key key) {
           if (place < out.top_k)
-            WriteTop(out, base + q * apart, place, key, from, sum, log_sum);
+            WriteTop<K>(out, base + q * apart, place, key, from, sum, log_sum);
         });
       }
     }
@@ -366,49 +455,50 @@ struct TokenShared {
   uint32_t bound;
   float all_high;  // of a block, for its cluster
   float2 all_sums;
-  float group[kTeam == 32 ? 1 : 4 * kTeam];
+  float group[kTeam == 32 ? 1 : kTeam];
+  int32_t places[kTeam == 32 ? 1 : 288];  // RoomFor(K2B200_MAX_TOP)
 };
 
 // The keys that the blocks of a cluster show each other.
 struct TokenTogether {
-  int32_t top;                       // keys in `list`
-  uint64_t list[K2B200_MAX_TOP];     // this block's, largest first
-  uint64_t others[7 * K2B200_MAX_TOP];
+  int32_t top;                    // keys in `list`
+  uint64_t list[K2B200_MAX_TOP];  // this block's, largest first
+  uint64_t lists[8][K2B200_MAX_TOP];
+  int32_t tops[8];
 };
 
 // The places of a row's keys where the blocks of a cluster have been through a slice each: every
-// block finds those of its own.
+// block finds those of its own, a thread for each of them and each list.
 __device__ __forceinline__ void PlaceTogether(const TokenOut &out, TokenTogether &together,
-                                              int32_t top_k, int32_t r, uint32_t cluster,
-                                              uint32_t rank, int32_t tid, int32_t team, float high,
-                                              float sum) {
+                                              int32_t *places, int32_t top_k, int32_t r,
+                                              uint32_t cluster, int32_t tid, int32_t team,
+                                              float high, float sum) {
+  using K = Keys<float, 512>;
   const float log_sum = logf(sum);
-  int32_t others = 0;
-  for (uint32_t b = 0; b < cluster; ++b) {
-    if (b == rank) continue;
-    const int32_t n = ReadFrom(&together.top, b);
-    for (int32_t k = tid; k < n; k += team)
-      together.others[others + k] = ReadFrom(&together.list[k], b);
-    others += n;
+  if (tid < (int32_t)cluster) together.tops[tid] = ReadFrom(&together.top, tid);
+  for (int32_t k = tid; k < top_k; k += team) places[k] = 0;
+  __syncthreads();
+  for (int32_t k = tid; k < (int32_t)cluster * K2B200_MAX_TOP; k += team) {
+    const int32_t b = k / K2B200_MAX_TOP, at = k % K2B200_MAX_TOP;
+    if (at < together.tops[b]) together.lists[b][at] = ReadFrom(&together.list[at], b);
   }
   __syncthreads();
-  for (int32_t k = tid; k < top_k; k += team) {
-    const uint64_t key = together.list[k];
-    int32_t place = k, begin = 0;
-    for (uint32_t b = 0; b < cluster; ++b) {
-      if (b == rank) continue;
-      // how many of a list that falls are larger
-      const int32_t n = ReadFrom(&together.top, b);
-      int32_t low = 0, far = n;
-      while (low < far) {
-        const int32_t mid = (low + far) / 2;
-        if (together.others[begin + mid] > key) low = mid + 1; else far = mid;
-      }
-      place += low;
-      begin += n;
+  for (int32_t k = tid; k < (int32_t)cluster * K2B200_MAX_TOP; k += team) {
+    const int32_t b = k / K2B200_MAX_TOP, at = k % K2B200_MAX_TOP;
+    if (at >= top_k) continue;
+    const uint64_t key = together.list[at];
+    // how many of a list that falls are larger
+    int32_t low = 0, far = together.tops[b];
+    while (low < far) {
+      const int32_t mid = (low + far) / 2;
+      if (together.lists[b][mid] > key) low = mid + 1; else far = mid;
     }
-    if (place < out.top_k) WriteTop(out, r, place, key, high, sum, log_sum);
+    if (low > 0) atomicAdd(&places[at], low);
   }
+  __syncthreads();
+  for (int32_t k = tid; k < top_k; k += team)
+    if (places[k] < out.top_k)
+      WriteTop<K>(out, r, places[k], together.list[k], high, sum, log_sum);
 }
 
 // Longer rows: a warp (kTeam 32, several to a block) or a block is a team, or a cluster of blocks
@@ -431,7 +521,9 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
   TokenShared<kTeam> &sh = all_shared[team];
   const int32_t stage = kTeam * vectors;
   uint4 *slot = shared + team * stage + tid;
-  uint64_t *keys = reinterpret_cast<uint64_t *>(shared + teams * stage) + team * out.room;
+  using K = Keys<T, kTeam>;
+  typename K::Key *keys =
+      reinterpret_cast<typename K::Key *>(shared + teams * stage) + team * out.room;
   const int32_t apart = (int32_t)(gridDim.x / cluster) * teams;
   const bool slopes = out.entropy || out.norm,
              speaks = rank == 0 && (kTeam == 32 || warp == 0);
@@ -522,10 +614,8 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
           sh.high[parity][warp] = high;
           sh.sums[parity][warp] = both;
         }
-        if (kTop) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) sh.group[g * kTeam + tid] = sums.group[g];
-        }
+        // (a block's threads are groups enough)
+        if (kTop) sh.group[tid] = sums.high;
         __syncthreads();
         // (without top classes or a cluster nobody else needs them)
         if (kTop || cluster > 1 || warp == 0) {
@@ -546,19 +636,24 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) four[g] = OrderOf(sums.group[g]);
           } else {
+            // (of 16 or 8 groups per lane four are made, or 8 for many classes)
 #pragma unroll
             for (int g = 0; g < 4; ++g) four[g] = 0;
-#pragma unroll 4
-            for (int g = 0; g < 4 * kTeam / 32; g += 4)
 #pragma unroll
-              for (int u = 0; u < 4; ++u)
-                four[u] = max(four[u], OrderOf(sh.group[32 * (g + u) + lane]));
+            for (int g = 0; g < kTeam / 32; ++g)
+              four[g & 3] = max(four[g & 3], OrderOf(sh.group[32 * g + lane]));
           }
           if (top_k <= 16) {
             const uint32_t one[1] = {max(max(four[0], four[1]), max(four[2], four[3]))};
             bound = BoundOf(one, top_k);
-          } else {
+          } else if (kTeam == 32 || top_k <= 64) {
             bound = BoundOf(four, top_k);
+          } else {
+            uint32_t eight[8] = {};
+#pragma unroll
+            for (int g = 0; g < kTeam / 32; ++g)
+              eight[g & 7] = max(eight[g & 7], OrderOf(sh.group[kTeam == 32 ? 0 : 32 * g + lane]));
+            bound = BoundOf(eight, top_k);
           }
           if (lane == 0) {
             sh.bound = bound;
@@ -594,14 +689,14 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
           if (tid == 0) sh.found = 0;
           TeamSync<kTeam>();
           EachKey<kTeam>(span, first, last, tid, bound,
-                         [&](uint64_t key) { keys[Count(&sh.found)] = key; });
+                         [&](uint64_t key) { keys[Count(&sh.found)] = K::From(key); });
           TeamSync<kTeam>();
           found = sh.found;
         }
       }
       if (kTeam == 512 && cluster > 1) {
         if constexpr (kTop && kTeam == 512) {
-          EachPlace(keys, found, tid, kTeam, [&](int32_t at, uint64_t key) {
+          EachPlaceBlock<kTeam>(keys, found, sh.places, tid, [&](int32_t at, uint64_t key) {
             if (at < top_k) together.list[at] = key;
           });
           if (tid == 0) together.top = top_k;
@@ -616,16 +711,21 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
         const float2 part = one ? ReadFrom(&sh.all_sums, lane) : make_float2(0.0f, 0.0f);
         both = JoinWarp(h, part, &high);
         if constexpr (kTop && kTeam == 512)
-          PlaceTogether(out, together, top_k, r, cluster, rank, tid, kTeam,
+          PlaceTogether(out, together, sh.places, top_k, r, cluster, tid, kTeam,
                         high == -INFINITY ? 0.0f : high, both.x);
         ClusterSync();  // nobody goes on while others read its memory
       } else if (kTop) {
         const float log_sum = logf(both.x), from = high == -INFINITY ? 0.0f : high;
-        EachPlace(keys, found, tid, kTeam, [&](int32_t at, uint64_t key) {
-          if (at < out.top_k) WriteTop(out, r, at, key, from, both.x, log_sum);
-        });
+        const auto write = [&](int32_t at, typename K::Key key) {
+          if (at < out.top_k) WriteTop<K>(out, r, at, key, from, both.x, log_sum);
+        };
         // (the next row's keys come to the same place, in a block behind two more barriers)
-        if (kTeam == 32) __syncwarp();
+        if constexpr (kTeam == 32) {
+          EachPlaceWarp(keys, found, lane, write);
+          __syncwarp();
+        } else {
+          EachPlaceBlock<kTeam>(keys, found, sh.places, tid, write);
+        }
       }
       if (lane == q) {
         my_high = high == -INFINITY ? 0.0f : high;
@@ -799,12 +899,15 @@ int32_t LaunchTokenScores(const k2b200_class_rows *rows, const TokenOut &out, cu
   const Rows<T> r = RowsOf<T>(rows);
   const int32_t key_bytes = (int32_t)sizeof(uint64_t) * out.room;
   const RowPlan p = PlanRows(r, key_bytes);
-  const size_t smem = (size_t)p.ring + (size_t)key_bytes * (p.block / p.team);
+  // (short rows with top classes: two of them, see TokenWarps)
+  const size_t smem = (size_t)p.ring * (p.in_registers && kTop ? 2 : 1) +
+                      (size_t)key_bytes * (p.block / p.team);
   if (p.in_registers) {
     auto kernel = p.vectors == 1   ? TokenWarps<T, 1, kTop>
                   : p.vectors == 2 ? TokenWarps<T, 2, kTop>
                   : p.vectors == 4 ? TokenWarps<T, 4, kTop>
                                    : TokenWarps<T, 8, kTop>;
+    K2B_CUDA_OK(AllowShared(kernel, smem));
     kernel<<<(uint32_t)p.blocks, p.block, smem, s>>>(r, out);
   } else {
     auto kernel = p.team == 32    ? TokenRing<T, 32, kTop>
