@@ -529,6 +529,74 @@ __device__ __forceinline__ void AddRow(Sums &s, uint4 *slot, int32_t mine, const
     then(slot, i);
   }
 }
+// A slice [first, last) of a row's vectors as a team of `team` threads reads it from memory: the whole
+// ones, and the ends that the row shares with its neighbours, which threads 0 and 1 have.
+template <typename T>
+struct RowStream {
+  RowSpan<T> span;
+  const uint4 *in;
+  int32_t first, last, from, to;
+  __device__ __forceinline__ RowStream(const RowSpan<T> &row, int32_t begin, int32_t end)
+      : span(row), in(reinterpret_cast<const uint4 *>(row.row - row.shift)), first(begin),
+        last(end) {
+    from = first < last && !span.Whole(span.Column(first)) ? first + 1 : first;
+    to = last > from && !span.Whole(span.Column(last - 1)) ? last - 1 : last;
+  }
+  // The vector at an end that this thread has, or -1.
+  __device__ __forceinline__ int32_t End(int32_t tid) const {
+    if (tid == 0 && from > first) return first;
+    if (tid == 1 && to < last && last - 1 >= from) return last - 1;
+    return -1;
+  }
+};
+// f(x, count, j): up to four of a thread's vectors at a time, j the first of them and a team's
+// width apart; the next four are read meanwhile.
+template <int kTeam, typename T, typename F>
+__device__ __forceinline__ void EachFour(const RowStream<T> &s, int32_t tid, F &&f) {
+#pragma unroll 1
+  for (int32_t j = s.from + tid; j < s.to; j += 4 * kTeam) {
+    uint4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (j + u * kTeam < s.to) x[u] = s.in[j + u * kTeam];
+    f(x, min(4, (s.to - j + kTeam - 1) / kTeam), j);
+  }
+}
+template <bool kSlope, int kTeam, typename T>
+__device__ __forceinline__ Sums SumStream(const RowStream<T> &stream, int32_t tid, float k) {
+  Sums s = NoSums();
+  const T *type = stream.span.row;
+  const auto one = [&](const uint4 &x, int u) {
+    const float high = VectorMax(x, type);
+    s.group[u] = fmaxf(s.group[u], high);
+    Raise<kSlope>(s, high, k);
+    AddVector<kSlope>(x, type, s.high == -INFINITY ? 0.0f : s.high, k, s.sum, s.slope);
+  };
+  EachFour<kTeam>(stream, tid, [&](uint4 (&x)[4], int32_t count, int32_t) {
+    if (count == 4) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s.group[u] = fmaxf(s.group[u], VectorMax(x[u], type));
+      Raise<kSlope>(s, fmaxf(fmaxf(s.group[0], s.group[1]), fmaxf(s.group[2], s.group[3])), k);
+      const float from = s.high == -INFINITY ? 0.0f : s.high;
+      Two sum = {0}, slope = {0};  // of every second vector
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        After(x[u], u & 1 ? sum : s.sum);
+        AddVector<kSlope>(x[u], type, from, k, u & 1 ? sum : s.sum, u & 1 ? slope : s.slope);
+      }
+      s.sum = Add(s.sum, sum);
+      if (kSlope) s.slope = Add(s.slope, slope);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 3; ++u)
+        if (u < count) one(x[u], u);
+    }
+  });
+  const int32_t end = stream.End(tid);
+  if (end >= 0) one(stream.span.Edge(end), 3);
+  return s;
+}
+
 // A warp's sums against its largest score.
 template <bool kSlope>
 __device__ __forceinline__ float2 WarpSums(const Sums &s, float k, float *high) {
@@ -550,6 +618,16 @@ __device__ __forceinline__ void Store(T *out, const RowSpan<T> &span, bool align
   const int32_t c0 = span.Column(j);
   if (aligned && span.Whole(c0)) {
     *reinterpret_cast<uint4 *>(out + c0) = Pack(f, out);
+    return;
+  }
+  // (words where pairs of scores are aligned)
+  if (aligned && kPer<T> == 8 && ((span.shift | span.classes) & 1) == 0) {
+    const uint4 v = Pack(f, out);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c0 + 2 * k >= 0 && c0 + 2 * k < span.classes)
+        *reinterpret_cast<uint32_t *>(out + c0 + 2 * k) = w[k];
     return;
   }
 #pragma unroll

@@ -36,22 +36,23 @@ __device__ __forceinline__ float TeacherScore(const Teacher &t, int64_t k) {
 }
 
 // Rows that count, of given lengths.  The kernel behind it starts meanwhile.
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(256)
 DistilCount(const void *lengths, int32_t lengths_64, int64_t outer, int64_t inner, double weight,
             DistilScale *scale) {
   LetNextStart();
-  __shared__ long long counted;
-  if (threadIdx.x == 0) counted = 0;
-  __syncthreads();
+  __shared__ long long counted[8];
   long long mine = 0;
-  for (int64_t o = threadIdx.x; o < outer; o += 1024) {
+  for (int64_t o = threadIdx.x; o < outer; o += 256) {
     const int64_t n = IntAt(lengths, lengths_64, o);
     mine += n < 0 ? 0 : n > inner ? inner : n;
   }
-  if (mine) atomicAdd(reinterpret_cast<unsigned long long *>(&counted), (unsigned long long)mine);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+  if ((threadIdx.x & 31) == 0) counted[threadIdx.x >> 5] = mine;
   __syncthreads();
   if (threadIdx.x == 0) {
-    scale->exact = weight / (double)(counted > 1 ? counted : 1);
+    for (int w = 1; w < 8; ++w) mine += counted[w];
+    scale->exact = weight / (double)(mine > 1 ? mine : 1);
     scale->rounded = (float)scale->exact;
   }
 }
@@ -800,7 +801,7 @@ int32_t LaunchDistil(const k2b200_class_rows *rows, const k2b200_teacher *t, flo
   double *partial =
       workspace ? reinterpret_cast<double *>(static_cast<char *>(workspace) + kDistilHead) : nullptr;
   if (by.device) {
-    DistilCount<<<1, 1024, 0, s>>>(rows->lengths, rows->lengths_64, rows->outer, rows->inner,
+    DistilCount<<<1, 256, 0, s>>>(rows->lengths, rows->lengths_64, rows->outer, rows->inner,
                                    t->weight, static_cast<DistilScale *>(workspace));
     NoteLaunch();
   }

@@ -333,7 +333,7 @@ TokenWarps(Rows<T> rows, TokenOut out) {
   typename K::Key *keys =
       reinterpret_cast<typename K::Key *>(shared + warps * kRows * kStage) + warp * out.room;
   const int32_t apart = (int32_t)gridDim.x * warps;
-  const bool slopes = out.entropy || out.norm;
+  const bool slopes = out.entropy != nullptr;
   for (int32_t base = (int32_t)blockIdx.x * warps + warp; base < rows.count; base += 32 * apart) {
     const int32_t mine = base + lane * apart,
                   taken = min(32, (rows.count - base + apart - 1) / apart);
@@ -501,6 +501,63 @@ __device__ __forceinline__ void PlaceTogether(const TokenOut &out, TokenTogether
       WriteTop<K>(out, r, places[k], together.list[k], high, sum, log_sum);
 }
 
+// Longer rows without top classes: a block is a team, or a cluster of blocks (kTeam 512); one pass.
+template <typename T, int kTeam>
+__global__ void __launch_bounds__(kTeam, kTeam == 512 ? 2 : 1280 / kTeam)
+TokenStream(Rows<T> rows, TokenOut out) {
+  __shared__ TokenShared<kTeam> sh;
+  const int32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t cluster = kTeam == 512 ? ClusterSize() : 1,
+                 rank = kTeam == 512 ? ClusterRank() : 0;
+  const int32_t r = (int32_t)(blockIdx.x / cluster);
+  const RowPlace at = PlaceOf(rows, r);
+  if (!at.counts) {
+    if (rank == 0 && tid == 0) SkipRow(out, r);
+    return;  // (all blocks of the cluster)
+  }
+  const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
+                        rows.classes);
+  const int32_t slice = (span.vectors + (int32_t)cluster - 1) / (int32_t)cluster;
+  const int32_t first = min(span.vectors, (int32_t)rank * slice);
+  const RowStream<T> stream(span, first, min(span.vectors, first + slice));
+  int64_t token = -1;
+  float score = 0.0f;
+  if (out.log_probs && rank == 0 && tid == 0) {
+    token = IntAt(out.tokens, out.tokens_64, r);
+    if (token >= 0 && token < rows.classes) score = ToFloat(span.row[token]);
+  }
+  float high;
+  float2 both =
+      out.entropy
+          ? WarpSums<true>(SumStream<true, kTeam>(stream, tid, kLog2e), kLog2e, &high)
+          : WarpSums<false>(SumStream<false, kTeam>(stream, tid, kLog2e), kLog2e, &high);
+  if (lane == 0) {
+    sh.high[0][warp] = high;
+    sh.sums[0][warp] = both;
+  }
+  __syncthreads();
+  if (warp > 0 && cluster == 1) return;
+  const bool one = lane < kTeam / 32;
+  both = JoinWarp(one ? sh.high[0][lane] : -INFINITY,
+                  one ? sh.sums[0][lane] : make_float2(0.0f, 0.0f), &high);
+  if (cluster > 1) {
+    if (tid == 0) {
+      sh.all_high = high;
+      sh.all_sums = both;
+    }
+    ClusterSync();
+    const bool other = lane < (int32_t)cluster;
+    if (rank == 0 && warp == 0) {
+      const float h = other ? ReadFrom(&sh.all_high, lane) : -INFINITY;
+      const float2 part = other ? ReadFrom(&sh.all_sums, lane) : make_float2(0.0f, 0.0f);
+      both = JoinWarp(h, part, &high);
+    }
+    ClusterSync();  // nobody leaves while others read its memory
+  }
+  if (rank == 0 && tid == 0)
+    Finish(out, r, rows.classes, token, score, high == -INFINITY ? 0.0f : high, both.x, both.y);
+}
+
 // Longer rows: a warp (kTeam 32, several to a block) or a block is a team, or a cluster of blocks
 // (kTeam 512), to which a row's vectors are dealt out in slices.  Rows come 32 at a time, as in
 // TokenWarps; the first warp of a row's first block computes what the rows have one of.  tiles > 1: a
@@ -525,7 +582,7 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
   typename K::Key *keys =
       reinterpret_cast<typename K::Key *>(shared + teams * stage) + team * out.room;
   const int32_t apart = (int32_t)(gridDim.x / cluster) * teams;
-  const bool slopes = out.entropy || out.norm,
+  const bool slopes = out.entropy != nullptr,
              speaks = rank == 0 && (kTeam == 32 || warp == 0);
   int32_t parity = 0;
   for (int32_t base = (int32_t)(blockIdx.x / cluster) * teams + team; base < rows.count;
@@ -786,66 +843,101 @@ struct Spread {
   }
 };
 
-// A team per row, or per part of `part` vectors of one: the norm is known, so every class is on its
-// own.  Four vectors per thread are read while the four before them are worked on.  The classes that
-// are a given or a top one are written again behind the others.
-template <typename T, int kTeam, bool kTop>
+// What the upstream and the norm say of a row.
+struct TokenRowGrad {
+  int32_t token;  // -1 for none
+  float token_grad, slope, top_sum;
+  float4 norm;
+};
+__device__ __forceinline__ TokenRowGrad ReadRowGrad(const TokenGrad &g, int32_t classes,
+                                                    const RowPlace &at, int32_t r) {
+  TokenRowGrad row;
+  row.norm = g.norm[r];
+  const int64_t token = g.log_probs.grad ? IntAt(g.tokens, g.tokens_64, r) : -1;
+  const bool some = token >= 0 && token < classes;
+  row.token = some ? (int32_t)token : -1;
+  row.token_grad = token == -1 ? 0.0f : some ? GradAt(g.log_probs, at) : NAN;
+  row.slope = GradAt(g.entropy, at);
+  row.top_sum = 0.0f;
+  return row;
+}
+__device__ __forceinline__ Spread SpreadOf(const TokenRowGrad &row, float top_sum) {
+  const float inverse = row.norm.y == 0.0f ? 0.0f : 1.0f / row.norm.y;
+  Spread spread;
+  spread.high = row.norm.x;
+  spread.by = -row.slope * inverse;
+  // (a row without a class left: no class has a share)
+  spread.constant =
+      row.norm.y == 0.0f
+          ? 0.0f
+          : -inverse * fmaf(row.slope, row.norm.z - logf(row.norm.y), row.token_grad + top_sum);
+  return spread;
+}
+// The given class, unless it is a top one, and the top classes, of those in [begin, end): by one warp
+// behind the stores of all others.
+template <bool kTop, typename T>
+__device__ __forceinline__ void WriteTokens(const TokenGrad &g, const TokenRowGrad &row,
+                                            const Spread &spread, const RowPlace &at, int32_t r,
+                                            const T *x, T *out, int32_t begin, int32_t end,
+                                            int32_t lane) {
+  bool is_top = false;
+  if (kTop) {
+    const int32_t *top = g.top_tokens + (int64_t)r * g.top_k;
+    for (int32_t k = lane; k < g.top_k; k += 32) {
+      const int32_t c = top[k];
+      is_top |= c == row.token;
+      if (c < begin || c >= end) continue;
+      float value = spread(ToFloat(x[c])) + GradAt(g.top, at, k);
+      if (c == row.token) value += row.token_grad;
+      out[c] = FromFloat<T>(value);
+    }
+    is_top = __any_sync(0xffffffffu, is_top);
+  }
+  if (lane == 0 && !is_top && row.token >= begin && row.token < end)
+    out[row.token] = FromFloat<T>(spread(ToFloat(x[row.token])) + row.token_grad);
+}
+
+// A block per part of `part` vectors of a row: the norm is known, so every class is on its own.  Four
+// vectors per thread are read while the four before them are worked on.  The classes that are a given
+// or a top one are written again behind the others.
+template <typename T, bool kTop>
 __global__ void __launch_bounds__(256, 4)
-TokenScoresBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t part) {
-  constexpr int kTile = 4;
-  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int32_t tid = kTeam == 32 ? lane : (int32_t)threadIdx.x;
-  const int32_t r = kTeam == 32 ? (int32_t)(blockIdx.x * (blockDim.x >> 5)) + warp
-                                : (int32_t)(blockIdx.x / (uint32_t)parts);
-  if (r >= rows.count) return;
-  const int32_t first = kTeam == 32 ? 0 : (int32_t)(blockIdx.x % (uint32_t)parts) * part;
+TokenBlocksBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t part) {
+  constexpr int kTeam = 256, kTile = 4;
+  const int32_t tid = threadIdx.x, lane = tid & 31;
+  const int32_t r = (int32_t)(blockIdx.x / (uint32_t)parts);
+  const int32_t first = (int32_t)(blockIdx.x % (uint32_t)parts) * part;
   const RowPlace at = PlaceOf(rows, r);
   T *out = grad + at.o * g.outer_stride + at.i * g.inner_stride;
   if (!at.counts) {
-    WriteZeros(out, rows.classes, first, kTeam == 32 ? INT32_MAX : first + part, tid, kTeam);
+    WriteZeros(out, rows.classes, first, first + part, tid, kTeam);
     return;
   }
   const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
                         rows.classes);
   const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
-  const int32_t last = kTeam == 32 ? span.vectors : min(span.vectors, first + part);
-  // vectors [from, to) are whole
-  const int32_t from = first < last && !span.Whole(span.Column(first)) ? first + 1 : first,
-                to = last > from && !span.Whole(span.Column(last - 1)) ? last - 1 : last;
-  const uint4 *in = reinterpret_cast<const uint4 *>(span.row - span.shift);
+  const RowStream<T> stream(span, min(first, span.vectors), min(span.vectors, first + part));
   uint4 v[kTile];
   const auto load = [&](int32_t tile) {
 #pragma unroll
     for (int i = 0; i < kTile; ++i)
-      if (tile + i * kTeam < to) v[i] = in[tile + i * kTeam];
+      if (tile + i * kTeam < stream.to) v[i] = stream.in[tile + i * kTeam];
   };
-  load(from + tid);
-  const float4 n = g.norm[r];
-  const int64_t token = g.log_probs.grad ? IntAt(g.tokens, g.tokens_64, r) : -1;
-  const bool some = token >= 0 && token < rows.classes;
-  const float token_grad = token == -1 ? 0.0f : some ? GradAt(g.log_probs, at) : NAN;
+  load(stream.from + tid);
+  const TokenRowGrad row = ReadRowGrad(g, rows.classes, at, r);
   float top_sum = 0.0f;
   if (kTop) {
     // (each warp for itself)
     for (int32_t k = lane; k < g.top_k; k += 32) top_sum += GradAt(g.top, at, k);
     top_sum = WarpSumF(top_sum);
   }
-  const float slope = GradAt(g.entropy, at), inverse = n.y == 0.0f ? 0.0f : 1.0f / n.y;
-  Spread spread;
-  spread.high = n.x;
-  spread.by = -slope * inverse;
-  // (a row without a class left: no class has a share)
-  spread.constant =
-      n.y == 0.0f ? 0.0f : -inverse * fmaf(slope, n.z - logf(n.y), token_grad + top_sum);
-  const auto store = [&](int32_t j, const uint4 &x, bool whole) {
+  const Spread spread = SpreadOf(row, top_sum);
+  const auto edge = [&](int32_t j, const uint4 &x) {
     float f[kPer<T>];
     spread(x, span.row, f);
-    if (whole && aligned)
-      *reinterpret_cast<uint4 *>(out + span.Column(j)) = Pack(f, out);
-    else
-      Store(out, span, false, j, f);
+    Store(out, span, false, j, f);
   };
-  for (int32_t tile = from + tid; tile < to; tile += kTeam * kTile) {
+  for (int32_t tile = stream.from + tid; tile < stream.to; tile += kTeam * kTile) {
     uint4 x[kTile];
 #pragma unroll
     for (int i = 0; i < kTile; ++i) x[i] = v[i];
@@ -853,39 +945,82 @@ TokenScoresBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t p
     if (aligned) {
 #pragma unroll
       for (int i = 0; i < kTile; ++i)
-        if (tile + i * kTeam < to) store(tile + i * kTeam, x[i], true);
+        if (tile + i * kTeam < stream.to) {
+          float f[kPer<T>];
+          spread(x[i], span.row, f);
+          *reinterpret_cast<uint4 *>(out + span.Column(tile + i * kTeam)) = Pack(f, out);
+        }
     } else {
 #pragma unroll 1
-      for (int32_t j = tile; j < min(to, tile + kTeam * kTile); j += kTeam) store(j, in[j], false);
+      for (int32_t j = tile; j < min(stream.to, tile + kTeam * kTile); j += kTeam)
+        edge(j, stream.in[j]);
     }
   }
-  // the row's ends
-  if (tid < 2) {
-    const int32_t j = tid == 0 ? first : last - 1;
-    if ((j < from || j >= to) && j < last && (tid == 0 || j > first)) store(j, span.Edge(j), false);
-  }
-  // behind the stores of the other threads: the token, unless a top class, and the top classes
-  TeamSync<kTeam>();
-  const int32_t begin = max(0, span.Column(first)),
-                end = min(span.classes, span.Column(last));
-  const auto mine = [&](int64_t c) { return c >= begin && c < end; };
-  bool token_is_top = false;
-  if (kTop) {
-    const int32_t *top = g.top_tokens + (int64_t)r * g.top_k;
-    for (int32_t k = tid; k < g.top_k; k += kTeam) {
-      const int32_t c = top[k];
-      if (!mine(c)) continue;
-      float value = spread(ToFloat(span.row[c])) + GradAt(g.top, at, k);
-      if (c == token) value += token_grad;
-      out[c] = FromFloat<T>(value);
+  const int32_t end_at = stream.End(tid);
+  if (end_at >= 0) edge(end_at, span.Edge(end_at));
+  // behind the stores of the other threads
+  __syncthreads();
+  const int32_t begin = max(0, span.Column(stream.first)),
+                end = min(span.classes, span.Column(stream.last));
+  if (tid < 32) WriteTokens<kTop>(g, row, spread, at, r, span.row, out, begin, end, lane);
+}
+
+// Short rows: a warp takes 32 of them, a whole grid of warps apart.  Lane q reads what there is to
+// know of the q-th, for all rows at once.
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(128, 6)
+TokenWarpsBackward(Rows<T> rows, TokenGrad g, T *grad) {
+  const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int32_t apart = (int32_t)gridDim.x * warps;
+  for (int32_t base = (int32_t)blockIdx.x * warps + warp; base < rows.count; base += 32 * apart) {
+    const int32_t mine = base + lane * apart,
+                  taken = min(32, (rows.count - base + apart - 1) / apart);
+    RowPlace my_at = {};
+    TokenRowGrad my_row = {};
+    T *my_out = nullptr;
+    if (lane < taken) {
+      my_at = PlaceOf(rows, mine);
+      my_out = grad + my_at.o * g.outer_stride + my_at.i * g.inner_stride;
+      if (my_at.counts) {
+        my_row = ReadRowGrad(g, rows.classes, my_at, mine);
+        if (kTop)
+          for (int32_t k = 0; k < g.top_k; ++k) my_row.top_sum += GradAt(g.top, my_at, k);
+      }
     }
-    if (some && tid < 32) {
-      for (int32_t k = lane; k < g.top_k; k += 32) token_is_top |= top[k] == token;
-      token_is_top = __any_sync(0xffffffffu, token_is_top);
+    const Spread my_spread = SpreadOf(my_row, my_row.top_sum);
+    const auto from = [&](auto v, int32_t q) { return __shfl_sync(0xffffffffu, v, q); };
+    for (int32_t q = 0; q < taken; ++q) {
+      T *out = reinterpret_cast<T *>(from(reinterpret_cast<unsigned long long>(my_out), q));
+      if (!from((int32_t)my_at.counts, q)) {
+        WriteZeros(out, rows.classes, 0, INT32_MAX, lane, 32);
+        continue;
+      }
+      RowPlace at;
+      at.o = from(my_at.o, q);
+      at.i = from(my_at.i, q);
+      TokenRowGrad row;
+      row.token = from(my_row.token, q);
+      row.token_grad = from(my_row.token_grad, q);
+      Spread spread;
+      spread.high = from(my_spread.high, q);
+      spread.constant = from(my_spread.constant, q);
+      spread.by = from(my_spread.by, q);
+      const RowSpan<T> span(rows.scores + at.o * rows.outer_stride + at.i * rows.inner_stride,
+                            rows.classes);
+      const bool aligned = (((uintptr_t)out ^ (uintptr_t)span.row) & 15) == 0;
+      const RowStream<T> stream(span, 0, span.vectors);
+#pragma unroll 2
+      for (int32_t j = lane; j < span.vectors; j += 32) {
+        const bool whole = j >= stream.from && j < stream.to;
+        const uint4 x = whole ? stream.in[j] : span.Edge(j);
+        float f[kPer<T>];
+        spread(x, span.row, f);
+        Store(out, span, aligned, j, f);
+      }
+      __syncwarp();
+      WriteTokens<kTop>(g, row, spread, at, base + q * apart, span.row, out, 0, rows.classes, lane);
     }
   }
-  if (tid == 0 && some && !token_is_top && mine(token))
-    out[token] = FromFloat<T>(spread(ToFloat(span.row[token])) + token_grad);
 }
 
 }  // namespace k2b
@@ -909,10 +1044,13 @@ int32_t LaunchTokenScores(const k2b200_class_rows *rows, const TokenOut &out, cu
                                    : TokenWarps<T, 8, kTop>;
     K2B_CUDA_OK(AllowShared(kernel, smem));
     kernel<<<(uint32_t)p.blocks, p.block, smem, s>>>(r, out);
+  } else if (!kTop && p.team > 32) {
+    K2B_CUDA_OK(LaunchRows(p.team == 256 ? TokenStream<T, 256> : TokenStream<T, 512>,
+                           (int64_t)r.count * p.cluster, p.block, 0, p.cluster, false, s, r, out));
   } else {
     auto kernel = p.team == 32    ? TokenRing<T, 32, kTop>
-                  : p.team == 256 ? TokenRing<T, 256, kTop>
-                                  : TokenRing<T, 512, kTop>;
+                  : p.team == 256 ? TokenRing<T, 256, true>
+                                  : TokenRing<T, 512, true>;
     K2B_CUDA_OK(AllowShared(kernel, smem));
     K2B_CUDA_OK(LaunchRows(kernel, p.blocks, p.block, smem, p.cluster, false, s, r, out, p.vectors,
                            p.tiles));
@@ -934,15 +1072,17 @@ int32_t LaunchTokenBackward(const k2b200_class_rows *rows, const TokenGrad &g, v
   const int32_t vectors = CeilDiv((int64_t)r.classes + kPer<T> - 1, kPer<T>) + 1;
   if (vectors <= 256) {
     const int32_t warps =
-        (int32_t)std::min<int64_t>(8, std::max<int64_t>(1, r.count / NumSms()));
-    auto kernel = top ? TokenScoresBackward<T, 32, true> : TokenScoresBackward<T, 32, false>;
-    kernel<<<CeilDiv(r.count, warps), 32 * warps, 0, s>>>(r, g, out, 1, 0);
+        (int32_t)std::min<int64_t>(4, std::max<int64_t>(1, r.count / NumSms()));
+    auto kernel = top ? TokenWarpsBackward<T, true> : TokenWarpsBackward<T, false>;
+    const int64_t blocks = std::min<int64_t>((r.count + warps - 1) / warps,
+                                             (int64_t)NumSms() * 6 * (4 / warps));
+    kernel<<<(uint32_t)blocks, 32 * warps, 0, s>>>(r, g, out);
   } else {
     const int32_t part = CeilDiv(vectors, 4096) * (int64_t)r.count >= 2 * NumSms() ? 4096 : 1024,
                   parts = CeilDiv(vectors, part);
     K2B_REQUIRE((int64_t)parts * r.count < ((int64_t)1 << 31), "too many rows of %d classes",
                 r.classes);
-    auto kernel = top ? TokenScoresBackward<T, 256, true> : TokenScoresBackward<T, 256, false>;
+    auto kernel = top ? TokenBlocksBackward<T, true> : TokenBlocksBackward<T, false>;
     kernel<<<(uint32_t)((int64_t)parts * r.count), 256, 0, s>>>(r, g, out, parts, part);
   }
   NoteLaunch();
