@@ -702,7 +702,7 @@ __device__ __forceinline__ V ReadFrom(const V *mine, uint32_t rank) {
 // ---------------------------------------------------------------------------
 // How the rows of a call are dealt out.
 struct RowPlan {
-  int32_t team;       // threads per row and block: 32, 256 or 512
+  int32_t team;       // threads per row and block: 32, 128, 256 or, in clusters, 512
   int32_t vectors;    // per thread: of a short row 1, 2, 4 or 8, which are registers; at most of others
   bool in_registers;
   int32_t cluster;    // blocks per row
@@ -733,10 +733,18 @@ static inline RowPlan PlanRows(const Rows<T> &r, int32_t more) {
     fit = (int64_t)ResidentBlocks(p.vectors) * (128 / p.block);
   } else {
     p.in_registers = false;
-    if (vectors <= 32 * 32 && rows >= 4 * (int64_t)sms) {
+    // What a team does once per row, each of its warps does: few threads and many vectors each, as
+    // long as enough rows fit an SM.  bf16 rows of 160 MB in all, us with 16 top classes / of a
+    // distillation, by threads to a row:
+    //           32         128        256        512
+    //   12 KB   64 /  76   81 / 122  121 / 188  199 / 352
+    //   24      79 /  87   66 /  87   83 / 122  116 / 198
+    //   48       -         57 /  75   66 /  86   77 / 132
+    //   80       -         73 /  96   59 /  77   63 / 105
+    if (vectors <= 32 * 36 && rows >= 4 * (int64_t)sms) {
       p.block = 128;
     } else {
-      p.team = p.block = 256;
+      p.team = p.block = vectors <= 128 * 28 ? 128 : 256;
       // over more SMs: rows that do not fit one, and few rows, down to 8 KB each
       while (p.cluster < 8 && (vectors * 16 > p.cluster * kShared * 7 / 8 ||
                                (rows * p.cluster * 2 <= sms && vectors > p.cluster * 2 * 512))) {

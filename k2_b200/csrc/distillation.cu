@@ -388,7 +388,7 @@ constexpr int32_t kHeld = kTeam == 32 ? 1 : 3;
 // tiles > 1: a slice does not fit, and is read again, part by part, for each pass.
 template <typename T, int kTeam>
 __global__ void
-__launch_bounds__(kTeam == 32 ? 128 : kTeam, kTeam == 32 ? 5 : kTeam == 256 ? 2 : 1)
+__launch_bounds__(kTeam == 32 ? 128 : kTeam, kTeam == 32 ? 5 : kTeam == 128 ? 4 : kTeam == 256 ? 2 : 1)
 DistilRing(Rows<T> rows, Teacher t, float4 *norm, float *loss, double *partial, T *grad,
            int64_t outer_stride, int64_t inner_stride, DistilBy by, int32_t vectors,
            int32_t tiles) {
@@ -826,6 +826,7 @@ int32_t LaunchDistil(const k2b200_class_rows *rows, const k2b200_teacher *t, flo
                                         : p.vectors == 4 ? DistilWarps<T, 4>
                                                          : DistilWarps<T, 8>)
                                : launch(p.team == 32    ? DistilRing<T, 32>
+                                        : p.team == 128 ? DistilRing<T, 128>
                                         : p.team == 256 ? DistilRing<T, 256>
                                                         : DistilRing<T, 512>,
                                         p.vectors, p.tiles));

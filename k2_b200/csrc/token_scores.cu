@@ -1045,10 +1045,13 @@ int32_t LaunchTokenScores(const k2b200_class_rows *rows, const TokenOut &out, cu
     K2B_CUDA_OK(AllowShared(kernel, smem));
     kernel<<<(uint32_t)p.blocks, p.block, smem, s>>>(r, out);
   } else if (!kTop && p.team > 32) {
-    K2B_CUDA_OK(LaunchRows(p.team == 256 ? TokenStream<T, 256> : TokenStream<T, 512>,
+    K2B_CUDA_OK(LaunchRows(p.team == 128   ? TokenStream<T, 128>
+                           : p.team == 256 ? TokenStream<T, 256>
+                                           : TokenStream<T, 512>,
                            (int64_t)r.count * p.cluster, p.block, 0, p.cluster, false, s, r, out));
   } else {
     auto kernel = p.team == 32    ? TokenRing<T, 32, kTop>
+                  : p.team == 128 ? TokenRing<T, 128, true>
                   : p.team == 256 ? TokenRing<T, 256, true>
                                   : TokenRing<T, 512, true>;
     K2B_CUDA_OK(AllowShared(kernel, smem));
