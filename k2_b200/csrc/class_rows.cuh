@@ -331,11 +331,12 @@ __device__ __forceinline__ uint4 Keep(const uint4 &v, int32_t begin, int32_t end
 template <typename T>
 struct RowPart {
   RowSpan<T> span;
-  int32_t first, last, mine;  // mine: this thread's
+  int32_t first, last, mine, most;  // mine: this thread's; most: any thread's
   __device__ __forceinline__ RowPart(const RowSpan<T> &row, int32_t from, int32_t to, int32_t tid,
                                      int32_t team)
       : span(row), first(from + tid), last(to) {
     mine = first < last ? (last - first + team - 1) / team : 0;
+    most = (to - from + team - 1) / team;
   }
 };
 
@@ -419,6 +420,8 @@ __device__ __forceinline__ void CutEnds(uint4 *slot, const RowPart<T> &part) {
     uint4 &v = slot[(part.mine - 1) * kTeam];
     v = Keep(v, 0, rest, span.row);
   }
+  // (as many for every thread, so that those of a warp go through a row together)
+  if (part.mine < part.most) slot[part.mine * kTeam] = LowestVector(span.row);
 }
 
 // Sums of 2^d and of d 2^d over a vector, d = (x - high) * k.

@@ -522,7 +522,7 @@ DistilRing(Rows<T> rows, Teacher t, float4 *norm, float *loss, double *partial, 
       // the largest score and the sum of each warp
       Sums sums = NoSums();
       each([&](const RowPart<T> &part) {
-        AddRow<false, kTeam>(sums, slot, part.mine, row, k, NoRefill());
+        AddRow<false, kTeam>(sums, slot, part.most, row, k, NoRefill());
       });
       float high, sum = WarpSums<false>(sums, k, &high).x;
       bool some = teacher.some, wrong = teacher.wrong;

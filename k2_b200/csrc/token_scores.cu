@@ -183,16 +183,16 @@ __device__ __forceinline__ void CollectRow(uint4 *slot, const RowPart<T> &part, 
                                            const F &then) {
   constexpr int kWord = 32 / kPer<T>;
 #pragma unroll 1
-  for (int32_t i0 = 0; i0 < part.mine; i0 += kWord) {
+  for (int32_t i0 = 0; i0 < part.most; i0 += kWord) {
     uint32_t bits = 0;
 #pragma unroll
     for (int u = 0; u < kWord; ++u)
-      if (i0 + u < part.mine)
+      if (i0 + u < part.most)
         bits |= Reaching(slot[(i0 + u) * kTeam], least, part.span.row) << (u * kPer<T>);
     PutKeys<kTeam>(bits, slot, part, i0, keys, room, found);
 #pragma unroll
     for (int u = 0; u < kWord; ++u)
-      if (i0 + u < part.mine) then(slot, i0 + u);
+      if (i0 + u < part.most) then(slot, i0 + u);
   }
 }
 
@@ -650,17 +650,17 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
         CutEnds<kTeam>(slot, part);
         if constexpr (kTop) {
           if (slopes)
-            AddRow<true, kTeam>(sums, slot, part.mine, row, kLog2e, NoRefill());
+            AddRow<true, kTeam>(sums, slot, part.most, row, kLog2e, NoRefill());
           else
-            AddRow<false, kTeam>(sums, slot, part.mine, row, kLog2e, NoRefill());
+            AddRow<false, kTeam>(sums, slot, part.most, row, kLog2e, NoRefill());
         } else {
           if (slopes)
-            AddRow<true, kTeam>(sums, slot, part.mine, row, kLog2e, refill);
+            AddRow<true, kTeam>(sums, slot, part.most, row, kLog2e, refill);
           else
-            AddRow<false, kTeam>(sums, slot, part.mine, row, kLog2e, refill);
+            AddRow<false, kTeam>(sums, slot, part.most, row, kLog2e, refill);
         }
       });
-      if (!kTop) refill.Rest(slot, whole.mine, then, rows);
+      if (!kTop) refill.Rest(slot, whole.most, then, rows);
       float high;
       float2 both = slopes ? WarpSums<true>(sums, kLog2e, &high)
                            : WarpSums<false>(sums, kLog2e, &high);
@@ -723,7 +723,7 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
           if (tiles > 1) CutEnds<kTeam>(slot, part);
           CollectRow<kTeam>(slot, part, least, keys, out.room, &sh.found, refill);
         });
-        refill.Rest(slot, whole.mine, then, rows);
+        refill.Rest(slot, whole.most, then, rows);
         TeamSync<kTeam>();
         found = sh.found;
         if (found > out.room) {
