@@ -718,9 +718,9 @@ struct RowPlan {
 // Blocks of an SM that the kernels for short rows are compiled for.
 constexpr int ResidentBlocks(int vectors) { return vectors > 4 ? 6 : 8; }
 
-// `more`: bytes of shared memory that a team takes besides.
+// more_warp, more_block: bytes of shared memory that a team takes besides.
 template <typename T>
-static inline RowPlan PlanRows(const Rows<T> &r, int32_t more) {
+static inline RowPlan PlanRows(const Rows<T> &r, int32_t more_warp, int32_t more_block) {
   RowPlan p = {32, 1, true, 1, 1, 32, 0, 0};
   const int64_t rows = r.count, size = sizeof(T);
   // its vectors: one more where it does not begin with one
@@ -764,7 +764,7 @@ static inline RowPlan PlanRows(const Rows<T> &r, int32_t more) {
   }
   const int64_t teams = p.block / p.team;
   p.ring = p.block * p.vectors * 16;
-  fit = std::min(fit, kShared / (p.ring + more * teams + 1024));
+  fit = std::min(fit, kShared / (p.ring + (p.team == 32 ? more_warp * teams : more_block) + 1024));
   p.blocks = std::min<int64_t>((rows + teams - 1) / teams * p.cluster,
                                sms * std::max<int64_t>(1, fit) / p.cluster * p.cluster);
   return p;

@@ -808,7 +808,7 @@ int32_t LaunchDistil(const k2b200_class_rows *rows, const k2b200_teacher *t, flo
   int32_t parts = 0;
   if (r.count > 0) {
     const int32_t held = t->entries * kEntryBytes;
-    const RowPlan p = PlanRows(r, kHeld<512> * held);
+    const RowPlan p = PlanRows(r, kHeld<32> * held, kHeld<512> * held);
     const size_t smem =
         (size_t)p.ring + (size_t)(p.team == 32 ? kHeld<32> : kHeld<512>) * held * (p.block / p.team);
     parts = (int32_t)(p.blocks / p.cluster);

@@ -1033,7 +1033,7 @@ template <typename T, bool kTop>
 int32_t LaunchTokenScores(const k2b200_class_rows *rows, const TokenOut &out, cudaStream_t s) {
   const Rows<T> r = RowsOf<T>(rows);
   const int32_t key_bytes = (int32_t)sizeof(uint64_t) * out.room;
-  const RowPlan p = PlanRows(r, key_bytes);
+  const RowPlan p = PlanRows(r, key_bytes, key_bytes);
   // (short rows with top classes: two of them, see TokenWarps)
   const size_t smem = (size_t)p.ring * (p.in_registers && kTop ? 2 : 1) +
                       (size_t)key_bytes * (p.block / p.team);
