@@ -215,10 +215,10 @@ void RefuseForwardMode(const at::Tensor &t) {
   TORCH_CHECK(!t._fw_grad(0).defined(), "k2_b200 has no forward-mode derivatives");
 }
 
-void RefuseSecondOrder(const variable_list &grads) {
-  for (const at::Tensor &g : grads)
-    TORCH_CHECK(!torch::autograd::compute_requires_grad(g),
-                "k2_b200 has no derivatives of second order (create_graph=True)");
+// (a gradient without a graph of its own would be taken for a constant)
+void RefuseSecondOrder() {
+  TORCH_CHECK(!at::GradMode::is_enabled(),
+              "k2_b200 has no derivatives of second order (create_graph=True)");
 }
 
 // ---------------------------------------------------------------------------
@@ -235,7 +235,7 @@ struct TokenNode : public torch::autograd::Node {
 
   variable_list apply(variable_list &&grads) override {
     variable_list out(1);
-    RefuseSecondOrder(grads);
+    RefuseSecondOrder();
     at::Tensor g_log_probs, g_entropy, g_top;
     if (log_probs_at >= 0) g_log_probs = grads[log_probs_at];
     if (entropy_at >= 0) g_entropy = grads[entropy_at];
@@ -363,7 +363,7 @@ struct DistilNode : public torch::autograd::Node {
     variable_list out(1);
     at::Tensor g = grads[0];
     if (!g.defined()) return out;
-    RefuseSecondOrder(grads);
+    RefuseSecondOrder();
     TORCH_CHECK(!released,
                 "the loss was already differentiated and its buffers freed (retain_graph=True "
                 "keeps them)");

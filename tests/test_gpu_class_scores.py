@@ -130,6 +130,98 @@ def test_top_classes_of_awkward_rows(classes, top_k):
                      backward=False)
 
 
+# rows enough for every way that they are dealt out: a warp each (short rows in registers, longer ones
+# in shared memory), blocks of several sizes, clusters, and rows that not even a cluster holds
+MANY = [(700, 2100), (600, 5003), (593, 9000), (600, 9300), (160, 20000), (150, 33333),
+        (149, 60001), (75, 40000), (2, 1000003)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,classes", MANY)
+def test_every_way_that_rows_are_dealt_out(rows, classes, dtype):
+    """All rows are computed, some of them looked at."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    wide = torch.randn(rows, classes + 1, device=DEV, generator=g).mul_(2).to(dtype)
+    pick = torch.unique(torch.cat([torch.arange(0, rows, max(1, rows // 12)),
+                                   torch.tensor([rows - 1])])).to(DEV)
+    token = ints(-1, classes, (rows,), 1).to(DEV)
+    tt = ints(0, classes, (rows, 40), 2).to(DEV)
+    tt[::3, 7:] = -1
+    tt[1] = -1
+    lp = torch.randn(rows, 40, device=DEV, generator=g)
+    live = torch.ones(rows, dtype=torch.bool)
+    live[2::7] = False
+    # (rows as sequences of one frame)
+    lengths = live.to(DEV, torch.int32)
+    up = {n: torch.randn(rows, *more, device=DEV, generator=g)
+          for n, more in (("log_probs", ()), ("entropy", ()), ("top_log_probs", (20,)))}
+    # adjacent rows, and rows of a wider matrix, whose gradient lies otherwise
+    for x in (wide.reshape(-1)[:rows * classes].view(rows, classes), wide[:, 1:]):
+        for top_k in (0, 20):
+            leaf = x[:, None].detach().requires_grad_(True)
+            got = k2.token_log_probs(leaf, token[:, None], top_k=top_k, entropy=True,
+                                     lengths=lengths)
+            names = ["log_probs", "entropy"] + (["top_log_probs"] if top_k else [])
+            grad, = torch.autograd.grad([getattr(got, n) for n in names], leaf,
+                                        [up[n][:, None] for n in names])
+            want, tol = tokens_reference(x[pick], token[pick], top_k, live[pick.cpu()],
+                                         {n: up[n][pick] for n in names})
+            for n in names:
+                assert_close(getattr(got, n)[pick, 0], want[n], tol[n], n)
+            if top_k:
+                assert torch.equal(got.top_tokens[pick, 0].cpu(), want["top_tokens"])
+            assert_close(grad[pick, 0], want["grad"], tol["grad"], "grad")
+            assert (grad[~live.to(DEV)] == 0).all()
+        for reduction, upstream in (("sum", None), ("none", up["entropy"])):
+            leaf = x[:, None].detach().requires_grad_(True)
+            loss = k2.distillation_loss(leaf, tt[:, None], lp[:, None], 2.0, 0.5, reduction,
+                                        lengths)
+            grad, = torch.autograd.grad(loss, leaf, None if upstream is None
+                                        else upstream[:, None])
+            want, tol = distil_reference(x[pick], tt[pick], lp[pick], 2.0, 0.5, reduction,
+                                         live[pick.cpu()],
+                                         None if upstream is None else upstream[pick])
+            assert_close(grad[pick, 0], want["grad"], tol["grad"], "grad")
+            assert (grad[~live.to(DEV)] == 0).all()
+            if reduction == "none":
+                each = loss.detach()
+                assert_close(loss[pick, 0], want["loss"], tol["loss"], "loss")
+        # the sum is that of the rows' own, which the same kernel computes (halving them is exact):
+        # added in 64 bits and rounded once, by half a step of float32
+        with torch.no_grad():
+            total = k2.distillation_loss(x[:, None], tt[:, None], lp[:, None], 2.0, 0.5, "sum",
+                                         lengths)
+        rows_sum = each.double().sum()
+        assert abs(float(total - rows_sum)) <= 2.0 ** -23 * float(each.double().abs().sum())
+
+
+@pytest.mark.parametrize("rows,classes", [(300007, 9), (160001, 33)])
+def test_more_rows_than_a_warp_takes_at_once(rows, classes):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(rows, classes, device=DEV, generator=g)
+    token = ints(0, classes, (rows,), 1).to(DEV)
+    tt = ints(0, classes, (rows, 3), 2).to(DEV)
+    lp = torch.randn(rows, 3, device=DEV, generator=g)
+    check_tokens(x, token, top_k=2)
+    check_distil(x, tt, lp, reduction="none")
+    check_distil(x, tt, lp, reduction="mean")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [40, 500, 501, 1000])
+def test_order_of_the_smallest_differences(classes, dtype):
+    """Subnormals, zeros of both signs and neighbours of a type are told apart as numbers are."""
+    g = torch.Generator().manual_seed(classes)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # the smallest subnormal
+    steps = torch.randint(-5, 6, (8, classes), generator=g).double()
+    rows = [steps * tiny, steps.clamp(max=0) * tiny, steps.sign() * 0.0,
+            1 + steps * torch.finfo(dtype).eps, -1 - steps * torch.finfo(dtype).eps]
+    x = torch.cat(rows).to(dtype)
+    assert ((x == 0).any(1) & (x != 0).any(1)).any()
+    for top_k in (1, 2, 7, 8, 9, 30):
+        check_tokens(x.to(DEV), None, top_k=top_k, entropy=False, backward=False)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("classes", [5, 77, 500, 5000, 33001])
 def test_rows_with_infinities_and_lowest_values(classes, dtype):
@@ -601,6 +693,11 @@ def test_refusals():
     loss = k2.distillation_loss(leaf, tt, lp)
     with pytest.raises(RuntimeError, match="second order"):
         torch.autograd.grad((loss * leaf.sum()), leaf, create_graph=True)
+    loss = k2.distillation_loss(leaf, tt, lp)
+    with pytest.raises(RuntimeError, match="second order"):
+        loss.backward(create_graph=True)
+    with pytest.raises(RuntimeError, match="second order"):
+        k2.token_log_probs(leaf, token).log_probs.sum().backward(create_graph=True)
 
 
 def test_a_module_with_settings():
