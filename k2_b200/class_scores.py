@@ -38,7 +38,7 @@ def token_log_probs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
       entropy: whether -sum_c p_c log p_c is wanted.
       lengths: [N] int32 or int64, on the CPU or the device, for logits [N, T, C]: frames from
         `lengths[n]` on are not read; they get 0 everywhere, -1 as top classes, and no
-        gradient.
+        gradient.  Those on the CPU are read at the call: a captured call keeps them.
 
     A logit of -inf is a class of probability 0; in a row without any other every log-prob is
     -inf and the entropy 0.  A row with NaN or +inf is NaN (NaN comes first among the top

@@ -148,7 +148,7 @@ RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengt
             host.data_ptr<int32_t>(), l.size(0), r.lengths.data_ptr<int32_t>(),
             c10::cuda::getCurrentCUDAStream(scores.device().index()).stream()));
     } else {
-      r.lengths = l.contiguous();
+      r.lengths = (l.is_neg() ? l.resolve_neg() : l).contiguous();
     }
     // (an address even where there are no sequences: lengths are given)
     r.rows.lengths = r.lengths.data_ptr();
@@ -162,7 +162,7 @@ at::Tensor Classes(const at::Tensor &t, const RowsOf &r, const char *what) {
   Require(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, what);
   RequireCuda(t, "tokens");
   Require(t.device() == r.scores.device(), "tokens must be on the device of the logits");
-  return t.contiguous();
+  return (t.is_neg() ? t.resolve_neg() : t).contiguous();
 }
 
 bool LeadingSizesAre(const at::Tensor &t, const at::Tensor &scores, int64_t more) {
@@ -219,6 +219,17 @@ void RefuseForwardMode(const at::Tensor &t) {
 void RefuseSecondOrder() {
   TORCH_CHECK(!at::GradMode::is_enabled(),
               "k2_b200 has no derivatives of second order (create_graph=True)");
+}
+
+// The capture that a stream is in, 0 for none.
+unsigned long long CaptureOf(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // (the legacy stream, while another one is captured)
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
 }
 
 // ---------------------------------------------------------------------------
@@ -356,6 +367,7 @@ struct DistilNode : public torch::autograd::Node {
   SavedVariable saved_scores, saved_tokens, saved_teacher, saved_lengths;
   k2b200_teacher teacher{};
   at::Tensor tokens, teacher_scores, norm, workspace, ready;  // ready: for an upstream of 1
+  unsigned long long capture = 0;  // that the forward pass was in
   bool released = false;
 
   variable_list apply(variable_list &&grads) override {
@@ -383,17 +395,20 @@ struct DistilNode : public torch::autograd::Node {
       if (g.is_neg()) g = g.resolve_neg();
       up.grad = g.data_ptr<float>();
     }
-    // what the forward pass made is given away once: whoever gets it may add to it
-    const bool made = ready.defined();
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    // What the forward pass made is given away once: whoever gets it may add to it.  And only if
+    // both passes are in one capture, or neither is in any: a forward pass that is replayed by
+    // itself would write to the gradient of an earlier one, and a backward pass would find there
+    // what its last replay left.
+    const bool made = ready.defined() && capture == CaptureOf(stream);
     out[0] = made ? std::move(ready) : NewGrad(rows);
-    ready = at::Tensor();
+    if (made) ready = at::Tensor();
     int64_t outer = 0, inner = 0;
     GradStrides(out[0], rows, &outer, &inner);
     const bool work = workspace.defined();
     Check(k2b200_distillation_backward(
         &rows.rows, &teacher, norm.data_ptr<float>(), &up, made, out[0].data_ptr(), outer, inner,
-        work ? workspace.data_ptr() : nullptr, work ? (size_t)workspace.numel() : 0,
-        c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+        work ? workspace.data_ptr() : nullptr, work ? (size_t)workspace.numel() : 0, stream));
     return out;
   }
   void release_variables() override {
@@ -469,11 +484,11 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
     }
     loss = t.reduction == 0 ? NewOn(scores.sizes().slice(0, scores.dim() - 1), at::kFloat, device)
                             : NewOn({}, at::kFloat, device);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     Check(k2b200_distillation(&r.rows, &t, loss.data_ptr<float>(),
                               graded ? norm.data_ptr<float>() : nullptr,
                               ready.defined() ? ready.data_ptr() : nullptr, outer, inner,
-                              work, bytes,
-                              c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+                              work, bytes, stream));
     if (graded) {
       node = std::shared_ptr<DistilNode>(new DistilNode(), torch::autograd::deleteNode);
       node->saved_scores = SavedVariable(scores, false);
@@ -486,6 +501,7 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
       node->norm = norm;
       node->workspace = workspace;
       node->ready = ready;
+      if (ready.defined()) node->capture = CaptureOf(stream);
       node->rows = std::move(r);
     }
   }

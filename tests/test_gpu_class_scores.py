@@ -651,6 +651,43 @@ def test_captured_and_replayed(shape, classes):
             assert all(torch.equal(a, b) for a, b in zip(out, plain(seed + 10 * k)))
 
 
+@pytest.mark.parametrize("classes", [300, 5000])
+def test_a_forward_pass_replayed_by_itself(classes):
+    """Its gradients are no part of it: those of one replay stay when the next one runs."""
+    tt, lp = teacher((3,), classes, 6)
+    tt, lp = tt.to(DEV), lp.to(DEV)
+    inputs = [scores((3, classes), torch.float32, seed).to(DEV) for seed in (1, 2)]
+    x = inputs[0].clone().requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = k2.distillation_loss(x, tt, lp)
+    got = []
+    for value in inputs:
+        x.data.copy_(value)  # (.data: the buffer of a captured call, no version)
+        graph.replay()
+        torch.cuda.synchronize()
+        got += torch.autograd.grad(loss, x, retain_graph=True)
+        torch.cuda.synchronize()
+    for grad, value in zip(got, inputs):
+        want, tol = distil_reference(value, tt, lp)
+        assert_close(grad, want["grad"], tol["grad"])
+
+
+@pytest.mark.parametrize("classes", [300, 5000])
+def test_passes_captured_one_by_one(classes):
+    """A backward pass that is replayed twice, with an upstream of 1 behind another one."""
+    tt, lp = teacher((3,), classes, 6)
+    tt, lp = tt.to(DEV), lp.to(DEV)
+    x = scores((3, classes), torch.float32).to(DEV).requires_grad_(True)
+    graphed = torch.cuda.make_graphed_callables(k2.DistillationLoss(), (x, tt, lp))
+    loss = graphed(x, tt, lp)
+    for up in (2.0, 1.0, 1.0):
+        got, = torch.autograd.grad(loss, x, torch.tensor(up, device=DEV), retain_graph=True)
+        want, tol = distil_reference(x.detach(), tt, lp, up=torch.tensor(up))
+        assert_close(got, want["grad"], tol["grad"])
+        got.fill_(7.0)
+
+
 def test_refusals():
     x = torch.zeros(2, 3, 8, device=DEV)
     token = torch.zeros(2, 3, dtype=torch.int64, device=DEV)
