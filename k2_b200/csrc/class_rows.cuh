@@ -553,7 +553,7 @@ struct RowStream {
   }
 };
 // f(x, count, j): up to four of a thread's vectors at a time, j the first of them and a team's
-// width apart; the next four are read meanwhile.
+// width apart.
 template <int kTeam, typename T, typename F>
 __device__ __forceinline__ void EachFour(const RowStream<T> &s, int32_t tid, F &&f) {
 #pragma unroll 1
@@ -818,6 +818,8 @@ static inline int32_t CheckRows(const k2b200_class_rows *rows) {
               "%lld x %lld rows: fewer than 2^28", (long long)rows->outer,
               (long long)rows->inner);
   K2B_REQUIRE(rows->scores != nullptr || rows->outer * rows->inner == 0, "NULL pointer");
+  K2B_REQUIRE((uintptr_t)rows->scores % (rows->type == K2B200_F32 ? 4 : 2) == 0,
+              "scores that are not aligned to their type");
   return kOk;
 }
 

@@ -2,11 +2,11 @@
 // gradient.
 //
 // With q = softmax(t / T) over a row's entries and p = softmax(x / T) over its classes, the loss is
-// T^2 sum_j q_j (log q_j - log p_j) and its gradient T (p_c - sum_j q_j [c = j]).  Distil hold the
-// row in registers (class_rows.cuh), so that loss and gradient take one read and one write of it;
-// the gradient is for an upstream of 1, and DistilBackward makes it again for another one.  All
-// classes are written as if the teacher had named none, whole vectors at a time, and its classes
-// again behind them.
+// T^2 sum_j q_j (log q_j - log p_j) and its gradient T (p_c - sum_j q_j [c = j]).  DistilWarps (rows
+// up to 4 KB) and DistilRing have the row on the chip, so that loss and gradient take one read and one
+// write of it; the gradient is for an upstream of 1, and DistilBackward makes it again for another
+// one.  All classes are written as if the teacher had named none, whole vectors at a time, and its
+// classes again behind them.
 #include "class_rows.cuh"
 
 namespace k2b {
@@ -252,7 +252,8 @@ __device__ __forceinline__ void WriteGradRow(const uint4 *slot, const RowPart<T>
 
 // Short rows: each warp is a team.  It takes 32 rows at a time, a whole grid of warps apart; lane q
 // knows where the q-th of them is and computes its loss.  loss: of the rows, or NULL and `partial`
-// has the sum of each block's rows.
+// has the sum of each block's rows.  Bound by instructions (690 a row, 72% of the issue slots): 64 x
+// 1000 rows of 500 bf16 classes with 16 entries, a fifth beyond their lengths, 48 us, 2.5 TB/s.
 template <typename T, int kVectors>
 __global__ void __launch_bounds__(128, ResidentBlocks(kVectors))
 DistilWarps(Rows<T> rows, Teacher t, float4 *norm, float *loss, double *partial, T *grad,
@@ -385,7 +386,9 @@ constexpr int32_t kHeld = kTeam == 32 ? 1 : 3;
 // DistilWarps; each block's first warp reads the teacher, and that of a row's first block computes
 // the losses.  A block has one barrier per row: behind it, the sums of all warps are there, and the
 // gradient of the row before has been stored, so that the teacher's classes can be written into it.
-// tiles > 1: a slice does not fit, and is read again, part by part, for each pass.
+// tiles > 1: a slice does not fit, and is read again, part by part, for each pass.  16000 x 5000 fp16
+// with 32 entries, a quarter beyond their lengths: 66 us, 4.3 TB/s; 4096 x 50021 bf16 with 64: 190 us,
+// 4.3 TB/s, with two blocks of 100 KB to an SM, whose 16 warps issue in 43% of the cycles.
 template <typename T, int kTeam>
 __global__ void
 __launch_bounds__(kTeam == 32 ? 128 : kTeam, kTeam == 32 ? 5 : kTeam == 128 ? 4 : kTeam == 256 ? 2 : 1)

@@ -1,13 +1,16 @@
 // Log-probs of given classes, entropies and top classes of rows of scores, and their gradient.
 //
-// TokenScores holds a row in registers (class_rows.cuh).  Sums: with d_c = (x_c - high) log2 e and
-// e_c = 2^d_c, log p_c = (x_c - high) - ln sum e, and the entropy is ln sum e - ln 2 (sum e d) /
-// sum e.  Top classes: the threads' largest scores are themselves scores of the row, so that the
-// k-th largest of them bounds the row's k-th largest from below, and few scores lie above it (of
-// n threads about n ln(n / (n - k))); those are collected in shared memory, and each one's place
-// is the number of larger ones.  Where more lie above it than there is room for - ties, or many
-// large scores in one thread - the bound is raised by bisection over (score, class), which no two
+// With d_c = (x_c - high) log2 e and e_c = 2^d_c: log p_c = (x_c - high) - ln sum e, and the entropy is
+// ln sum e - ln 2 (sum e d) / sum e.  Top classes: the threads' largest scores are themselves scores of
+// the row, so that the k-th largest of them bounds the row's k-th largest from below, and few scores
+// lie above it (of n threads about n ln(n / (n - k))); those are collected in shared memory, and each
+// one's place is the number of larger ones.  Where more lie above it than there is room for - ties, or
+// many large scores in one thread - the bound is raised by bisection over (score, class), which no two
 // classes share.
+//
+// Kernels, by the length of a row (PlanRows): TokenWarps up to 4 KB, TokenRing with a warp per row up
+// to 18 KB, then with blocks where top classes are asked for, and TokenStream where not; few long rows
+// are dealt out to clusters.  TokenWarpsBackward and TokenBlocksBackward for the gradient.
 #include "class_rows.cuh"
 
 #include <type_traits>
@@ -319,7 +322,9 @@ __device__ __forceinline__ void EachPlaceBlock(const uint64_t *keys, int32_t n, 
 
 // Short rows: each warp is a team.  It takes 32 rows at a time, a whole grid of warps apart; lane q
 // knows where the q-th of them is and its given class, gathers its sums, and computes what a row
-// has one of, for all of them at once.
+// has one of, for all of them at once.  Bound by instructions: of 64 x 1000 rows of 500 bf16 classes,
+// a fifth of them beyond their lengths, 46 us for log-probs, entropy and 8 top classes (600
+// instructions a row, 340 of them for the top classes; three quarters of the issue slots), 1.2 TB/s.
 template <typename T, int kVectors, bool kTop>
 __global__ void __launch_bounds__(128, ResidentBlocks(kVectors))
 TokenWarps(Rows<T> rows, TokenOut out) {
@@ -501,7 +506,10 @@ __device__ __forceinline__ void PlaceTogether(const TokenOut &out, TokenTogether
       WriteTop<K>(out, r, places[k], together.list[k], high, sum, log_sum);
 }
 
-// Longer rows without top classes: a block is a team, or a cluster of blocks (kTeam 512); one pass.
+// Longer rows without top classes: a block is a team, or a cluster of blocks (kTeam 512); one pass over
+// the memory, without a copy of the row.  4096 x 32001 bf16 with entropy: 63 us, 4.2 TB/s, bound by
+// instructions and 2^d (11.8 instructions and one such per score, of 16 a cycle); without entropy
+// 6666 x 12000 take 32 us, 5.1 TB/s.
 template <typename T, int kTeam>
 __global__ void __launch_bounds__(kTeam, kTeam == 512 ? 2 : 1280 / kTeam)
 TokenStream(Rows<T> rows, TokenOut out) {
@@ -561,7 +569,10 @@ TokenStream(Rows<T> rows, TokenOut out) {
 // Longer rows: a warp (kTeam 32, several to a block) or a block is a team, or a cluster of blocks
 // (kTeam 512), to which a row's vectors are dealt out in slices.  Rows come 32 at a time, as in
 // TokenWarps; the first warp of a row's first block computes what the rows have one of.  tiles > 1: a
-// slice does not fit, and is read again, part by part, for each pass.
+// slice does not fit, and is read again, part by part, for each pass.  16000 x 5000 fp16 with 32 top
+// classes: 64 us, 2.6 TB/s, two thirds of the issue slots with the 20 warps that the rows' 10 KB leave
+// room for (36 us without top classes).  3 x 131072 fp32 with 64 on clusters of 8: 11 us, a chain of
+// reads, barriers and searches.
 template <typename T, int kTeam, bool kTop>
 __global__ void
 __launch_bounds__(kTeam == 32 ? 128 : kTeam, kTeam <= 128 ? 6 : kTeam == 256 ? 3 : 2)
@@ -899,7 +910,8 @@ __device__ __forceinline__ void WriteTokens(const TokenGrad &g, const TokenRowGr
 
 // A block per part of `part` vectors of a row: the norm is known, so every class is on its own.  Four
 // vectors per thread are read while the four before them are worked on.  The classes that are a given
-// or a top one are written again behind the others.
+// or a top one are written again behind the others.  4096 x 32001 bf16: 77 us, 6.8 TB/s read and
+// written, the memory's rate.
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(256, 4)
 TokenBlocksBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t part) {
@@ -966,7 +978,8 @@ TokenBlocksBackward(Rows<T> rows, TokenGrad g, T *grad, int32_t parts, int32_t p
 }
 
 // Short rows: a warp takes 32 of them, a whole grid of warps apart.  Lane q reads what there is to
-// know of the q-th, for all rows at once.
+// know of the q-th, for all rows at once.  24000 rows of 29 fp32 classes with 3 top classes: 12 us (a
+// warp per row that reads all of it for itself: 21).
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(128, 6)
 TokenWarpsBackward(Rows<T> rows, TokenGrad g, T *grad) {
