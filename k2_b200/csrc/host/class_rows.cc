@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
@@ -232,6 +233,23 @@ unsigned long long CaptureOf(cudaStream_t stream) {
   return status == cudaStreamCaptureStatusNone ? 0 : id;
 }
 
+// A leaf's gradient is added on the stream on which its first graph was made.  If that is the default
+// one, which no capture can wait for, a captured backward pass would break its capture there, in a
+// thread of torch's that ends the process.
+void RefuseLeafOfDefaultStream(const torch::autograd::Node &node, cudaStream_t stream) {
+  if (CaptureOf(stream) == 0) return;
+  for (const auto &edge : node.next_edges()) {
+    const auto leaf = dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get());
+    if (leaf == nullptr) continue;
+    const auto its = leaf->stream();
+    TORCH_CHECK(!its.has_value() || c10::cuda::CUDAStream(*its) !=
+                                        c10::cuda::getDefaultCUDAStream(its->device_index()),
+                "a backward pass cannot be captured while another graph of the same logits lives "
+                "that was made on the default stream: delete what holds it, or make it on another "
+                "stream");
+  }
+}
+
 // ---------------------------------------------------------------------------
 // token_log_probs
 // ---------------------------------------------------------------------------
@@ -263,6 +281,8 @@ struct TokenNode : public torch::autograd::Node {
     const at::Device device = rows.scores.device();
     c10::cuda::CUDAGuard guard(device);
     at::AutoDispatchBelowADInplaceOrView below_autograd;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    RefuseLeafOfDefaultStream(*this, stream);
     const k2b200_row_grad a = RowGrad(g_log_probs, rows, false),
                           b = RowGrad(g_entropy, rows, false), c = RowGrad(g_top, rows, true);
     out[0] = NewGrad(rows);
@@ -272,8 +292,7 @@ struct TokenNode : public torch::autograd::Node {
         &rows.rows, tokens.defined() ? tokens.data_ptr() : nullptr,
         tokens.defined() && tokens.scalar_type() == at::kLong, top_k,
         top_k > 0 ? top.data_ptr<int32_t>() : nullptr, norm.data_ptr<float>(), &a, &b, &c,
-        out[0].data_ptr(), outer, inner,
-        c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+        out[0].data_ptr(), outer, inner, stream));
     return out;
   }
   void release_variables() override {
@@ -387,6 +406,8 @@ struct DistilNode : public torch::autograd::Node {
     const at::Device device = rows.scores.device();
     c10::cuda::CUDAGuard guard(device);
     at::AutoDispatchBelowADInplaceOrView below_autograd;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    RefuseLeafOfDefaultStream(*this, stream);
     k2b200_row_grad up{};
     if (teacher.reduction == 0) {
       up = RowGrad(g, rows, false);
@@ -395,7 +416,6 @@ struct DistilNode : public torch::autograd::Node {
       if (g.is_neg()) g = g.resolve_neg();
       up.grad = g.data_ptr<float>();
     }
-    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     // What the forward pass made is given away once: whoever gets it may add to it.  And only if
     // both passes are in one capture, or neither is in any: a forward pass that is replayed by
     // itself would write to the gradient of an earlier one, and a backward pass would find there

@@ -1,4 +1,5 @@
 """`token_log_probs` and `distillation_loss` on the GPU against their definitions in 64 bits."""
+import gc
 import itertools
 import math
 
@@ -686,6 +687,31 @@ def test_passes_captured_one_by_one(classes):
         want, tol = distil_reference(x.detach(), tt, lp, up=torch.tensor(up))
         assert_close(got, want["grad"], tol["grad"])
         got.fill_(7.0)
+
+
+def test_a_captured_backward_pass_beside_a_graph_of_the_same_leaf():
+    """Refused where that graph was made on the default stream; the capture goes on, and the other
+    graph is what it was."""
+    tt, lp = teacher((3,), 300, 6)
+    tt, lp = tt.to(DEV), lp.to(DEV)
+    x = scores((3, 300), torch.float32).to(DEV).requires_grad_(True)
+    for call in (lambda: k2.distillation_loss(x, tt, lp),
+                 lambda: k2.token_log_probs(x, tt[:, 0]).log_probs.sum()):
+        other = call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = call()
+            with pytest.raises(RuntimeError, match="another graph of the same logits"):
+                torch.autograd.grad(loss, x)
+        want, = torch.autograd.grad(other, x)
+        del loss, other, graph
+        gc.collect()  # (what was raised refers to them)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            grad, = torch.autograd.grad(call(), x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
 
 
 def test_refusals():
