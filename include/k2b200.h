@@ -857,8 +857,8 @@ typedef struct {
 /* tokens [rows] (NULL: none are asked for): -1 has log-prob 0, any other that is no class NaN.
  * log_probs, entropy [rows] (each may be NULL); top_log_probs, top_tokens [rows, top_k], largest
  * first, a lower class before a higher one of the same score, NaN before all numbers.  A row that
- * does not count gets log-probs and entropy 0 and top_tokens -1.  norm [rows, 4]: for the
- * backward pass (NULL: none follows). */
+ * does not count gets log-probs and entropy 0 and top_tokens -1.  norm [rows, 4], 16-byte
+ * aligned: for the backward pass (NULL: none follows). */
 int32_t k2b200_token_scores(const k2b200_class_rows *rows, const void *tokens, int32_t tokens_64,
                             int32_t top_k, float *log_probs, float *entropy,
                             float *top_log_probs, int32_t *top_tokens, float *norm,

@@ -886,6 +886,9 @@ int32_t k2b200_distillation(const k2b200_class_rows *rows, const k2b200_teacher 
                             int64_t grad_outer_stride, int64_t grad_inner_stride,
                             void *workspace, size_t workspace_bytes, void *stream) {
   K2B_FORWARD(CheckRows(rows));
+  K2B_REQUIRE((uintptr_t)norm % 16 == 0, "norm that is not aligned to 16 bytes");
+  K2B_REQUIRE((uintptr_t)grad_scores % (rows->type == K2B200_F32 ? 4 : 2) == 0,
+              "a gradient that is not aligned to its type");
   K2B_FORWARD(CheckTeacher(teacher, rows));
   K2B_REQUIRE(!grad_scores || teacher->reduction != 0,
               "the gradient of row losses needs their upstream");
@@ -913,6 +916,9 @@ int32_t k2b200_distillation_backward(const k2b200_class_rows *rows, const k2b200
                                      const void *workspace, size_t workspace_bytes,
                                      void *stream) {
   K2B_FORWARD(CheckRows(rows));
+  K2B_REQUIRE((uintptr_t)norm % 16 == 0, "norm that is not aligned to 16 bytes");
+  K2B_REQUIRE((uintptr_t)grad_scores % (rows->type == K2B200_F32 ? 4 : 2) == 0,
+              "a gradient that is not aligned to its type");
   K2B_FORWARD(CheckTeacher(teacher, rows));
   if (rows->outer * rows->inner == 0) return kOk;
   const size_t need = teacher->reduction == 0 ? 0 : kDistilHead;

@@ -92,6 +92,17 @@ def test_distillation_calls_that_are_refused():
     assert distil_backward(rows(), teacher(), size=7) == TOO_SMALL
 
 
+def test_addresses_that_are_not_aligned_are_refused():
+    odd, half = rows(scores=FAR + 1, type=1), rows(scores=FAR + 2)
+    for status in (token_scores(odd), token_scores(half), token_backward(odd), distil(odd, teacher()),
+                   distil_backward(half, teacher()), token_backward(rows(), norm=FAR + 8),
+                   token_backward(rows(), grad=FAR + 2), token_backward(rows(type=2), grad=FAR + 1),
+                   distil(rows(), teacher(), grad=FAR + 2),
+                   distil_backward(rows(), teacher(), norm=FAR + 8),
+                   distil_backward(rows(), teacher(), grad=FAR + 2)):
+        assert status == INVALID and b"aligned" in _lib.lib.k2b200_last_error()
+
+
 def test_no_rows_are_no_work():
     empty = rows(outer=0, scores=None)
     assert token_scores(empty) == 0 and token_backward(empty) == 0
