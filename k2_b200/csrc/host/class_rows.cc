@@ -263,6 +263,7 @@ struct TokenNode : public torch::autograd::Node {
   bool released = false;
 
   variable_list apply(variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     RefuseSecondOrder();
     at::Tensor g_log_probs, g_entropy, g_top;
@@ -296,6 +297,7 @@ struct TokenNode : public torch::autograd::Node {
     return out;
   }
   void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
     released = true;
     saved_scores.reset_data();
     saved_tokens.reset_data();
