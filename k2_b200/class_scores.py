@@ -69,7 +69,8 @@ def distillation_loss(logits: torch.Tensor, teacher_tokens: torch.Tensor,
         0 where there are none), or "none": [...].
       lengths: as in `token_log_probs`; frames beyond them give no loss and no gradient.
 
-    A row without an entry, or with none of finite teacher_log_probs, gives 0 and no gradient.
+    A row without an entry, or with none above -inf, gives 0 and no gradient; one with NaN or +inf
+    among its entries is NaN.
 
     With "sum" and "mean" the gradient is made beside the loss, while a row is at hand, for an
     upstream of 1, and made again from the logits where the upstream is another: a factor of the

@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t BoundOf(const uint32_t (&order)[kGroups], in
 }
 
 // The keys that a team collects: score and class in one number (OrderOf), which sorts as they do.
-// A warp's rows have at most 8192 classes, so that with a score of 16 bits a key is one of 32.
+// A warp's rows have at most 32 * 36 * 8 classes, so that with a score of 16 bits a key is one of 32.
 template <typename T, int kTeam>
 struct Keys {
   using Key = uint64_t;
@@ -223,7 +223,8 @@ template <typename F>
 __device__ __forceinline__ uint64_t RaiseBound(uint64_t bound, int32_t top_k, int32_t room,
                                                int32_t classes, F &&count) {
   uint64_t low = bound, far = ~0ull, mid = bound + (1ull << 32);
-  for (;;) {
+  // (halved 64 times at most; the limit is for scores that somebody else changes meanwhile)
+  for (int32_t k = 0; k < 128; ++k) {
     const int32_t n = count(mid);
     if (n >= top_k && n <= room) return mid;
     if (n < top_k) far = mid; else low = mid;
@@ -232,6 +233,13 @@ __device__ __forceinline__ uint64_t RaiseBound(uint64_t bound, int32_t top_k, in
       low = max((unsigned long long)low, (low | 0xffffffffull) - (uint64_t)classes);
     mid = low + (far - low) / 2;
   }
+  return mid;
+}
+// Puts a key where there is room, as there is for all that reach such a bound.
+template <typename Key>
+__device__ __forceinline__ void PutKey(Key key, Key *keys, int32_t room, int32_t *found) {
+  const int32_t at = Count(found);
+  if (at < room) keys[at] = key;
 }
 
 template <typename K>
@@ -431,9 +439,11 @@ TokenWarps(Rows<T> rows, TokenOut out) {
           if (lane == 0) all_found[warp] = 0;
           __syncwarp();
           EachKey<32>(span, 0, span.vectors, lane, bound,
-                      [&](uint64_t key) { keys[Count(&all_found[warp])] = K::From(key); });
+                      [&](uint64_t key) {
+                        PutKey(K::From(key), keys, out.room, &all_found[warp]);
+                      });
           __syncwarp();
-          found = all_found[warp];
+          found = min(all_found[warp], out.room);
         }
         const float log_sum = logf(sum);
         EachPlaceWarp(keys, found, lane, [&](int32_t place, typename K::Key key) {
@@ -579,7 +589,8 @@ __launch_bounds__(kTeam == 32 ? 128 : kTeam, kTeam <= 128 ? 6 : kTeam == 256 ? 3
 TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
   extern __shared__ uint4 shared[];
   __shared__ TokenShared<kTeam> all_shared[kTeam == 32 ? 4 : 1];
-  __shared__ typename std::conditional<kTop && kTeam == 512, TokenTogether, int32_t>::type together;
+  static_assert(kTop || kTeam == 32, "TokenStream");
+  __shared__ typename std::conditional<kTeam == 512, TokenTogether, int32_t>::type together;
   const int32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31,
                 teams = kTeam == 32 ? (int32_t)blockDim.x / 32 : 1,
                 team = kTeam == 32 ? warp : 0,
@@ -683,15 +694,12 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
           sh.sums[parity][warp] = both;
         }
         // (a block's threads are groups enough)
-        if (kTop) sh.group[tid] = sums.high;
+        sh.group[tid] = sums.high;
         __syncthreads();
-        // (without top classes or a cluster nobody else needs them)
-        if (kTop || cluster > 1 || warp == 0) {
-          const bool one = lane < kTeam / 32;
-          const float h = one ? sh.high[parity][lane] : -INFINITY;
-          const float2 part = one ? sh.sums[parity][lane] : make_float2(0.0f, 0.0f);
-          both = JoinWarp(h, part, &high);
-        }
+        const bool one = lane < kTeam / 32;
+        const float h = one ? sh.high[parity][lane] : -INFINITY;
+        const float2 part = one ? sh.sums[parity][lane] : make_float2(0.0f, 0.0f);
+        both = JoinWarp(h, part, &high);
       }
       int32_t found = 0;
       const int32_t top_k = max(0, min(out.top_k, min(span.classes, span.Column(last)) -
@@ -757,13 +765,13 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
           if (tid == 0) sh.found = 0;
           TeamSync<kTeam>();
           EachKey<kTeam>(span, first, last, tid, bound,
-                         [&](uint64_t key) { keys[Count(&sh.found)] = K::From(key); });
+                         [&](uint64_t key) { PutKey(K::From(key), keys, out.room, &sh.found); });
           TeamSync<kTeam>();
-          found = sh.found;
+          found = min(sh.found, out.room);
         }
       }
       if (kTeam == 512 && cluster > 1) {
-        if constexpr (kTop && kTeam == 512) {
+        if constexpr (kTeam == 512) {
           EachPlaceBlock<kTeam>(keys, found, sh.places, tid, [&](int32_t at, uint64_t key) {
             if (at < top_k) together.list[at] = key;
           });
@@ -778,7 +786,7 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
         const float h = one ? ReadFrom(&sh.all_high, lane) : -INFINITY;
         const float2 part = one ? ReadFrom(&sh.all_sums, lane) : make_float2(0.0f, 0.0f);
         both = JoinWarp(h, part, &high);
-        if constexpr (kTop && kTeam == 512)
+        if constexpr (kTeam == 512)
           PlaceTogether(out, together, sh.places, top_k, r, cluster, tid, kTeam,
                         high == -INFINITY ? 0.0f : high, both.x);
         ClusterSync();  // nobody goes on while others read its memory
