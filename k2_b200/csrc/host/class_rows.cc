@@ -3,6 +3,7 @@
 // computes; the work is k2b200_token_scores* and k2b200_distillation* (include/k2b200.h).
 #include "class_rows.h"
 
+#include <ATen/SavedTensorHooks.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -84,6 +85,39 @@ int64_t SizeOf(const at::Tensor &t, int64_t from, int64_t to) {
   return n;
 }
 
+// A tensor as adjacent numbers: itself, or a copy.
+at::Tensor Plain(const at::Tensor &t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+
+// What a node keeps of a tensor between the passes: hooks of the caller may hold it elsewhere, so
+// that nothing else here may.  It may come back with other strides, but is read as what it was.
+class Saved {
+ public:
+  void Keep(const at::Tensor &t) {
+    variable_ = SavedVariable(t, false);
+    sizes_ = t.sizes().vec();
+    type_ = t.scalar_type();
+    device_ = t.device();
+    there_ = true;
+  }
+  bool there() const { return there_; }
+  at::Device device() const { return device_; }
+  at::Tensor Get() const {
+    const at::Tensor t = variable_.unpack();
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.sizes() == sizes_ &&
+                    t.scalar_type() == type_ && t.device() == device_,
+                "hooks gave back a saved tensor of other sizes, type or device than they got");
+    return t;
+  }
+  void Release() { variable_.reset_data(); }
+
+ private:
+  SavedVariable variable_;
+  std::vector<int64_t> sizes_;
+  at::ScalarType type_ = at::kFloat;
+  at::Device device_ = at::kCPU;
+  bool there_ = false;
+};
+
 // k2b200_class_rows of a tensor of scores, and what it points to.  The rows are the dimensions
 // before the last, the first `split` of them the outer ones.
 struct RowsOf {
@@ -93,8 +127,7 @@ struct RowsOf {
 };
 
 // Scores of adjacent classes whose rows lie at two strides are read in place, others are copied.
-// (kept: the tensor outlives the call and must not hold on to the graph)
-RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengths, bool kept) {
+RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengths) {
   RequireCuda(scores, "logits");
   Require(scores.dim() >= 1 && FloatType(scores) >= 0,
           "logits must be [..., classes] of float32, float16 or bfloat16");
@@ -102,8 +135,7 @@ RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengt
           "logits must have 1 to 2^30 classes");
   const int64_t lead = scores.dim() - 1;
   RowsOf r;
-  r.scores = kept ? scores.detach() : scores;
-  if (r.scores.is_neg()) r.scores = r.scores.resolve_neg();
+  r.scores = scores.is_neg() ? scores.resolve_neg() : scores;
   int64_t outer_stride = 0, inner_stride = 0;
   const auto splits = [&](int64_t s) {
     return OneStride(r.scores, 0, s, &outer_stride) &&
@@ -149,7 +181,7 @@ RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengt
             host.data_ptr<int32_t>(), l.size(0), r.lengths.data_ptr<int32_t>(),
             c10::cuda::getCurrentCUDAStream(scores.device().index()).stream()));
     } else {
-      r.lengths = (l.is_neg() ? l.resolve_neg() : l).contiguous();
+      r.lengths = Plain(l);
     }
     // (an address even where there are no sequences: lengths are given)
     r.rows.lengths = r.lengths.data_ptr();
@@ -163,7 +195,7 @@ at::Tensor Classes(const at::Tensor &t, const RowsOf &r, const char *what) {
   Require(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, what);
   RequireCuda(t, "tokens");
   Require(t.device() == r.scores.device(), "tokens must be on the device of the logits");
-  return (t.is_neg() ? t.resolve_neg() : t).contiguous();
+  return Plain(t);
 }
 
 bool LeadingSizesAre(const at::Tensor &t, const at::Tensor &scores, int64_t more) {
@@ -212,6 +244,16 @@ at::Tensor NewGrad(const RowsOf &r) {
   return grad;
 }
 
+// The norm of a forward pass, which is read in vectors of 16 bytes.
+at::Tensor NormOf(const Saved &norm) {
+  const at::Tensor t = Plain(norm.Get());
+  return (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone();
+}
+
+c10::optional<at::Tensor> LengthsOf(const Saved &lengths) {
+  return lengths.there() ? c10::optional<at::Tensor>(lengths.Get()) : c10::nullopt;
+}
+
 void RefuseForwardMode(const at::Tensor &t) {
   TORCH_CHECK(!t._fw_grad(0).defined(), "k2_b200 has no forward-mode derivatives");
 }
@@ -254,9 +296,7 @@ void RefuseLeafOfDefaultStream(const torch::autograd::Node &node, cudaStream_t s
 // token_log_probs
 // ---------------------------------------------------------------------------
 struct TokenNode : public torch::autograd::Node {
-  RowsOf rows;  // (the scores are read again: `saved` complains if they have been changed)
-  SavedVariable saved_scores, saved_tokens, saved_top, saved_lengths;
-  at::Tensor tokens, norm;
+  Saved scores, lengths, tokens, top, norm;
   int32_t top_k = 0;
   // which output the gradients arrive for
   int32_t log_probs_at = -1, entropy_at = -1, top_at = -1;
@@ -275,38 +315,36 @@ struct TokenNode : public torch::autograd::Node {
                 "the scores were already differentiated and their buffers freed "
                 "(retain_graph=True keeps them)");
     if (!task_should_compute_output(0)) return out;
-    saved_scores.unpack();
-    if (tokens.defined()) saved_tokens.unpack();
-    if (rows.lengths.defined()) saved_lengths.unpack();
-    const at::Tensor top = top_k > 0 ? saved_top.unpack() : at::Tensor();
-    const at::Device device = rows.scores.device();
+    // (hooks run here, under no guard of ours)
+    const at::Tensor x = scores.Get();
+    const c10::optional<at::Tensor> l = LengthsOf(lengths);
+    at::Tensor given = g_log_probs.defined() ? tokens.Get() : at::Tensor(),
+               classes = g_top.defined() ? top.Get() : at::Tensor();
+    const at::Device device = scores.device();
     c10::cuda::CUDAGuard guard(device);
     at::AutoDispatchBelowADInplaceOrView below_autograd;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     RefuseLeafOfDefaultStream(*this, stream);
-    const k2b200_row_grad a = RowGrad(g_log_probs, rows, false),
-                          b = RowGrad(g_entropy, rows, false), c = RowGrad(g_top, rows, true);
-    out[0] = NewGrad(rows);
+    const RowsOf r = MakeRows(x, l);
+    const at::Tensor n = NormOf(norm);
+    if (given.defined()) given = Plain(given);
+    if (classes.defined()) classes = Plain(classes);
+    const k2b200_row_grad a = RowGrad(g_log_probs, r, false), b = RowGrad(g_entropy, r, false),
+                          c = RowGrad(g_top, r, true);
+    out[0] = NewGrad(r);
     int64_t outer = 0, inner = 0;
-    GradStrides(out[0], rows, &outer, &inner);
+    GradStrides(out[0], r, &outer, &inner);
     Check(k2b200_token_scores_backward(
-        &rows.rows, tokens.defined() ? tokens.data_ptr() : nullptr,
-        tokens.defined() && tokens.scalar_type() == at::kLong, top_k,
-        top_k > 0 ? top.data_ptr<int32_t>() : nullptr, norm.data_ptr<float>(), &a, &b, &c,
-        out[0].data_ptr(), outer, inner, stream));
+        &r.rows, given.defined() ? given.data_ptr() : nullptr,
+        given.defined() && given.scalar_type() == at::kLong, top_k,
+        classes.defined() ? classes.data_ptr<int32_t>() : nullptr, n.data_ptr<float>(), &a, &b,
+        &c, out[0].data_ptr(), outer, inner, stream));
     return out;
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     released = true;
-    saved_scores.reset_data();
-    saved_tokens.reset_data();
-    saved_top.reset_data();
-    saved_lengths.reset_data();
-    rows.scores.reset();
-    rows.lengths.reset();
-    tokens.reset();
-    norm.reset();
+    for (Saved *t : {&scores, &lengths, &tokens, &top, &norm}) t->Release();
   }
 };
 
@@ -318,16 +356,15 @@ py::tuple TokenLogProbs(const at::Tensor &scores, const c10::optional<at::Tensor
   c10::cuda::CUDAGuard guard(device);
   RefuseForwardMode(scores);
   const bool graded = torch::autograd::compute_requires_grad(scores);
-  at::Tensor log_probs, entropy, top_log_probs, top_tokens;
-  std::shared_ptr<TokenNode> node;
+  at::Tensor log_probs, entropy, top_log_probs, top_tokens, tokens, norm;
+  RowsOf r;
   {
     at::AutoDispatchBelowADInplaceOrView below_autograd;
-    RowsOf r = MakeRows(scores, lengths, graded);
+    r = MakeRows(scores, lengths);
     Require(top_k >= 0 && top_k <= K2B200_MAX_TOP && top_k <= scores.size(-1),
             "top_k must be 0 to 128, and at most the number of classes");
     Require(given.has_value() || top_k > 0 || want_entropy,
             "nothing is asked for: give tokens, top_k or entropy");
-    at::Tensor tokens;
     if (given.has_value()) {
       Require(LeadingSizesAre(*given, scores, 0), "tokens must have the shape of logits[..., 0]");
       tokens = Classes(*given, r, "tokens must be int32 or int64");
@@ -341,7 +378,6 @@ py::tuple TokenLogProbs(const at::Tensor &scores, const c10::optional<at::Tensor
       top_log_probs = NewOn(lead_top, at::kFloat, device);
       top_tokens = NewOn(lead_top, at::kInt, device);
     }
-    at::Tensor norm;
     if (graded) norm = NewOn({r.rows.outer * r.rows.inner, 4}, at::kFloat, device);
     const auto floats = [](at::Tensor &t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
@@ -351,19 +387,15 @@ py::tuple TokenLogProbs(const at::Tensor &scores, const c10::optional<at::Tensor
                               floats(top_log_probs),
                               top_tokens.defined() ? top_tokens.data_ptr<int32_t>() : nullptr,
                               floats(norm), stream));
-    if (graded) {
-      node = std::shared_ptr<TokenNode>(new TokenNode(), torch::autograd::deleteNode);
-      node->saved_scores = SavedVariable(scores, false);
-      if (tokens.defined()) node->saved_tokens = SavedVariable(*given, false);
-      if (top_k > 0) node->saved_top = SavedVariable(top_tokens, false);
-      if (r.lengths.defined()) node->saved_lengths = SavedVariable(*lengths, false);
-      node->tokens = tokens;
-      node->norm = norm;
-      node->top_k = (int32_t)top_k;
-      node->rows = std::move(r);
-    }
   }
-  if (node) {
+  if (graded) {
+    const std::shared_ptr<TokenNode> node(new TokenNode(), torch::autograd::deleteNode);
+    node->scores.Keep(r.scores);
+    if (r.lengths.defined()) node->lengths.Keep(r.lengths);
+    if (tokens.defined()) node->tokens.Keep(tokens);
+    if (top_k > 0) node->top.Keep(top_tokens);
+    node->norm.Keep(norm);
+    node->top_k = (int32_t)top_k;
     node->set_next_edges(torch::autograd::collect_next_edges(scores));
     int32_t k = 0;
     for (auto [t, at] : {std::pair{&log_probs, &node->log_probs_at},
@@ -384,10 +416,9 @@ py::tuple TokenLogProbs(const at::Tensor &scores, const c10::optional<at::Tensor
 // distillation_loss
 // ---------------------------------------------------------------------------
 struct DistilNode : public torch::autograd::Node {
-  RowsOf rows;
-  SavedVariable saved_scores, saved_tokens, saved_teacher, saved_lengths;
+  Saved scores, lengths, tokens, teacher_scores, norm;
   k2b200_teacher teacher{};
-  at::Tensor tokens, teacher_scores, norm, workspace, ready;  // ready: for an upstream of 1
+  at::Tensor workspace, ready;  // ready: for an upstream of 1
   unsigned long long capture = 0;  // that the forward pass was in
   bool released = false;
 
@@ -401,18 +432,25 @@ struct DistilNode : public torch::autograd::Node {
                 "the loss was already differentiated and its buffers freed (retain_graph=True "
                 "keeps them)");
     if (!task_should_compute_output(0)) return out;
-    saved_scores.unpack();
-    saved_tokens.unpack();
-    saved_teacher.unpack();
-    if (rows.lengths.defined()) saved_lengths.unpack();
-    const at::Device device = rows.scores.device();
+    // (hooks run here, under no guard of ours)
+    const at::Tensor x = scores.Get();
+    const c10::optional<at::Tensor> l = LengthsOf(lengths);
+    at::Tensor classes = tokens.Get(), of_teacher = teacher_scores.Get();
+    const at::Device device = scores.device();
     c10::cuda::CUDAGuard guard(device);
     at::AutoDispatchBelowADInplaceOrView below_autograd;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     RefuseLeafOfDefaultStream(*this, stream);
+    const RowsOf r = MakeRows(x, l);
+    const at::Tensor n = NormOf(norm);
+    classes = Plain(classes);
+    of_teacher = Plain(of_teacher);
+    k2b200_teacher t = teacher;
+    t.tokens = classes.data_ptr();
+    t.scores = of_teacher.data_ptr();
     k2b200_row_grad up{};
-    if (teacher.reduction == 0) {
-      up = RowGrad(g, rows, false);
+    if (t.reduction == 0) {
+      up = RowGrad(g, r, false);
     } else {
       if (g.scalar_type() != at::kFloat) g = g.to(at::kFloat);
       if (g.is_neg()) g = g.resolve_neg();
@@ -423,26 +461,22 @@ struct DistilNode : public torch::autograd::Node {
     // itself would write to the gradient of an earlier one, and a backward pass would find there
     // what its last replay left.
     const bool made = ready.defined() && capture == CaptureOf(stream);
-    out[0] = made ? std::move(ready) : NewGrad(rows);
+    out[0] = made ? std::move(ready) : NewGrad(r);
     if (made) ready = at::Tensor();
     int64_t outer = 0, inner = 0;
-    GradStrides(out[0], rows, &outer, &inner);
+    GradStrides(out[0], r, &outer, &inner);
     const bool work = workspace.defined();
     Check(k2b200_distillation_backward(
-        &rows.rows, &teacher, norm.data_ptr<float>(), &up, made, out[0].data_ptr(), outer, inner,
+        &r.rows, &t, n.data_ptr<float>(), &up, made, out[0].data_ptr(), outer, inner,
         work ? workspace.data_ptr() : nullptr, work ? (size_t)workspace.numel() : 0, stream));
     return out;
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     released = true;
-    saved_scores.reset_data();
-    saved_tokens.reset_data();
-    saved_teacher.reset_data();
-    saved_lengths.reset_data();
-    rows.scores.reset();
-    rows.lengths.reset();
-    for (at::Tensor *t : {&tokens, &teacher_scores, &norm, &workspace, &ready}) t->reset();
+    for (Saved *t : {&scores, &lengths, &tokens, &teacher_scores, &norm}) t->Release();
+    workspace.reset();
+    ready.reset();
   }
 };
 
@@ -455,12 +489,13 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
   c10::cuda::CUDAGuard guard(device);
   RefuseForwardMode(scores);
   const bool graded = torch::autograd::compute_requires_grad(scores);
-  at::Tensor loss;
-  std::shared_ptr<DistilNode> node;
+  at::Tensor loss, tokens, teacher_scores, workspace, norm, ready;
+  RowsOf r;
+  k2b200_teacher t{};
+  unsigned long long capture = 0;
   {
     at::AutoDispatchBelowADInplaceOrView below_autograd;
-    RowsOf r = MakeRows(scores, lengths, graded);
-    k2b200_teacher t{};
+    r = MakeRows(scores, lengths);
     t.reduction = reduction == "none" ? 0 : reduction == "sum" ? 1 : reduction == "mean" ? 2 : -1;
     Require(t.reduction >= 0, "reduction must be \"none\", \"sum\" or \"mean\"");
     // (1e-6 to 1e6 as float32: beyond them the scaled scores overflow)
@@ -470,8 +505,7 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
             "teacher_tokens must be [..., entries] over the rows of the logits");
     const int64_t entries = teacher_tokens.size(-1);
     Require(entries >= 1 && entries <= K2B200_MAX_TOP, "a teacher has 1 to 128 entries per row");
-    const at::Tensor tokens =
-        Classes(teacher_tokens, r, "teacher_tokens must be int32 or int64");
+    tokens = Classes(teacher_tokens, r, "teacher_tokens must be int32 or int64");
     Require(teacher_log_probs.sizes() == teacher_tokens.sizes() &&
                 FloatType(teacher_log_probs) >= 0,
             "teacher_log_probs must be float32, float16 or bfloat16 of the shape of "
@@ -482,9 +516,7 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
     // (a silent zero is what a caller who wants that derivative would get)
     Require(!(at::GradMode::is_enabled() && teacher_log_probs.requires_grad()),
             "no gradient goes to teacher_log_probs: detach them");
-    at::Tensor teacher_scores = teacher_log_probs.detach();
-    if (teacher_scores.is_neg()) teacher_scores = teacher_scores.resolve_neg();
-    teacher_scores = teacher_scores.contiguous();
+    teacher_scores = Plain(teacher_log_probs);
     t.tokens = tokens.data_ptr();
     t.tokens_64 = tokens.scalar_type() == at::kLong;
     t.scores = teacher_scores.data_ptr();
@@ -495,12 +527,12 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
     const int64_t num = r.rows.outer * r.rows.inner;
     // (rows' own losses need none)
     const size_t bytes = t.reduction == 0 ? 0 : k2b200_distillation_workspace_bytes(&r.rows);
-    at::Tensor workspace, norm, ready;
     if (bytes > 0) workspace = NewOn({(int64_t)bytes}, at::kByte, device);
     void *const work = bytes > 0 ? workspace.data_ptr() : nullptr;
     if (graded) norm = NewOn({num, 4}, at::kFloat, device);
     int64_t outer = 0, inner = 0;
-    if (graded && t.reduction != 0) {
+    // (whoever has hooks wants nothing large kept between the passes)
+    if (graded && t.reduction != 0 && !at::SavedTensorDefaultHooks::get_hooks().has_value()) {
       ready = NewGrad(r);
       GradStrides(ready, r, &outer, &inner);
     }
@@ -511,23 +543,19 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
                               graded ? norm.data_ptr<float>() : nullptr,
                               ready.defined() ? ready.data_ptr() : nullptr, outer, inner,
                               work, bytes, stream));
-    if (graded) {
-      node = std::shared_ptr<DistilNode>(new DistilNode(), torch::autograd::deleteNode);
-      node->saved_scores = SavedVariable(scores, false);
-      node->saved_tokens = SavedVariable(teacher_tokens, false);
-      node->saved_teacher = SavedVariable(teacher_log_probs, false);
-      if (r.lengths.defined()) node->saved_lengths = SavedVariable(*lengths, false);
-      node->teacher = t;
-      node->tokens = tokens;
-      node->teacher_scores = teacher_scores;
-      node->norm = norm;
-      node->workspace = workspace;
-      node->ready = ready;
-      if (ready.defined()) node->capture = CaptureOf(stream);
-      node->rows = std::move(r);
-    }
+    if (ready.defined()) capture = CaptureOf(stream);
   }
-  if (node) {
+  if (graded) {
+    const std::shared_ptr<DistilNode> node(new DistilNode(), torch::autograd::deleteNode);
+    node->scores.Keep(r.scores);
+    if (r.lengths.defined()) node->lengths.Keep(r.lengths);
+    node->tokens.Keep(tokens);
+    node->teacher_scores.Keep(teacher_scores);
+    node->norm.Keep(norm);
+    node->teacher = t;
+    node->workspace = workspace;
+    node->ready = ready;
+    node->capture = capture;
     node->set_next_edges(torch::autograd::collect_next_edges(scores));
     torch::autograd::set_history(loss, node);
   }
