@@ -771,11 +771,16 @@ static inline RowPlan PlanRows(const Rows<T> &r, int32_t more_warp, int32_t more
 }
 
 // Lets a kernel have more shared memory than the 48 KB that it has without asking (of which the
-// kernels here name up to 17 themselves).
+// kernels here name up to 17 themselves).  The limit is the kernel's, whichever thread of the host
+// sets it: every call sets the same one, for the longest ring of PlanRows with what a team has
+// besides, so that none takes away what another one is about to launch with.
+constexpr size_t kMostShared = 204 << 10;
 template <typename... Params>
 static cudaError_t AllowShared(void (*kernel)(Params...), size_t bytes) {
   if (bytes <= 30 << 10) return cudaSuccess;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (bytes > kMostShared) return cudaErrorInvalidValue;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)kMostShared);
 }
 
 // A launch of `blocks` blocks in clusters; `behind`: see LaunchBehind (common.cuh).
