@@ -833,6 +833,7 @@ int32_t k2b200_peer_reduce_status(void *local_buf, void *stream, int32_t *status
  *
  * A row holds the scores x of C classes, log p_c = x_c - log sum exp x.  Of NaN and +inf among
  * them comes NaN; a class of score -inf has p = 0, and where all have it, every log p is -inf.
+ * Arrays are aligned to their elements (norm to 16 bytes, a workspace to 8).
  * ------------------------------------------------------------------------- */
 typedef enum { K2B200_F32 = 0, K2B200_F16 = 1, K2B200_BF16 = 2 } k2b200_float_type;
 /* top_k of token scores, classes per row of a teacher */

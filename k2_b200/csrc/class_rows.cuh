@@ -809,6 +809,11 @@ static cudaError_t LaunchRows(void (*kernel)(Params...), int64_t blocks, int32_t
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// Whether an array of elements of `size` bytes, if there is one, lies as the device reads it.
+static inline bool Aligned(const void *array, size_t size) { return (uintptr_t)array % size == 0; }
+static inline size_t IntSize(int32_t is_64) { return is_64 ? 8 : 4; }
+static inline size_t FloatSize(int32_t type) { return type == K2B200_F32 ? 4 : 2; }
+
 // What the entry points ask of a k2b200_class_rows.
 static inline int32_t CheckRows(const k2b200_class_rows *rows) {
   K2B_REQUIRE(rows != nullptr, "NULL pointer");
@@ -823,8 +828,9 @@ static inline int32_t CheckRows(const k2b200_class_rows *rows) {
               "%lld x %lld rows: fewer than 2^28", (long long)rows->outer,
               (long long)rows->inner);
   K2B_REQUIRE(rows->scores != nullptr || rows->outer * rows->inner == 0, "NULL pointer");
-  K2B_REQUIRE((uintptr_t)rows->scores % (rows->type == K2B200_F32 ? 4 : 2) == 0,
-              "scores that are not aligned to their type");
+  K2B_REQUIRE(Aligned(rows->scores, FloatSize(rows->type)) &&
+                  Aligned(rows->lengths, IntSize(rows->lengths_64)),
+              "scores or lengths that are not aligned to their type");
   return kOk;
 }
 

@@ -773,6 +773,8 @@ int32_t CheckTeacher(const k2b200_teacher *t, const k2b200_class_rows *rows) {
               t->temperature);
   K2B_REQUIRE(t->reduction >= 0 && t->reduction <= 2, "unknown reduction %d", t->reduction);
   K2B_REQUIRE((t->tokens && t->scores) || rows->outer * rows->inner == 0, "NULL pointer");
+  K2B_REQUIRE(Aligned(t->tokens, IntSize(t->tokens_64)) && Aligned(t->scores, FloatSize(t->type)),
+              "a teacher's tokens or scores that are not aligned to their type");
   return kOk;
 }
 
@@ -886,9 +888,10 @@ int32_t k2b200_distillation(const k2b200_class_rows *rows, const k2b200_teacher 
                             int64_t grad_outer_stride, int64_t grad_inner_stride,
                             void *workspace, size_t workspace_bytes, void *stream) {
   K2B_FORWARD(CheckRows(rows));
-  K2B_REQUIRE((uintptr_t)norm % 16 == 0, "norm that is not aligned to 16 bytes");
-  K2B_REQUIRE((uintptr_t)grad_scores % (rows->type == K2B200_F32 ? 4 : 2) == 0,
-              "a gradient that is not aligned to its type");
+  K2B_REQUIRE(Aligned(norm, 16) && Aligned(workspace, sizeof(double)),
+              "norm or workspace that are not aligned to 16 and 8 bytes");
+  K2B_REQUIRE(Aligned(grad_scores, FloatSize(rows->type)) && Aligned(loss, 4),
+              "a loss or gradient that is not aligned to its type");
   K2B_FORWARD(CheckTeacher(teacher, rows));
   K2B_REQUIRE(!grad_scores || teacher->reduction != 0,
               "the gradient of row losses needs their upstream");
@@ -916,8 +919,9 @@ int32_t k2b200_distillation_backward(const k2b200_class_rows *rows, const k2b200
                                      const void *workspace, size_t workspace_bytes,
                                      void *stream) {
   K2B_FORWARD(CheckRows(rows));
-  K2B_REQUIRE((uintptr_t)norm % 16 == 0, "norm that is not aligned to 16 bytes");
-  K2B_REQUIRE((uintptr_t)grad_scores % (rows->type == K2B200_F32 ? 4 : 2) == 0,
+  K2B_REQUIRE(Aligned(norm, 16) && Aligned(workspace, sizeof(double)),
+              "norm or workspace that are not aligned to 16 and 8 bytes");
+  K2B_REQUIRE(Aligned(grad_scores, FloatSize(rows->type)) && Aligned(upstream ? upstream->grad : nullptr, 4),
               "a gradient that is not aligned to its type");
   K2B_FORWARD(CheckTeacher(teacher, rows));
   if (rows->outer * rows->inner == 0) return kOk;

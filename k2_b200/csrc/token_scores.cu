@@ -1123,7 +1123,10 @@ int32_t k2b200_token_scores(const k2b200_class_rows *rows, const void *tokens, i
                             float *top_log_probs, int32_t *top_tokens, float *norm,
                             void *stream) {
   K2B_FORWARD(CheckRows(rows));
-  K2B_REQUIRE((uintptr_t)norm % 16 == 0, "norm that is not aligned to 16 bytes");
+  K2B_REQUIRE(Aligned(norm, 16), "norm that is not aligned to 16 bytes");
+  K2B_REQUIRE(Aligned(tokens, IntSize(tokens_64)) && Aligned(log_probs, 4) &&
+                  Aligned(entropy, 4) && Aligned(top_log_probs, 4) && Aligned(top_tokens, 4),
+              "tokens or outputs that are not aligned to their type");
   K2B_REQUIRE(top_k >= 0 && top_k <= K2B200_MAX_TOP && top_k <= rows->num_classes,
               "top_k is %d: 0 to %d, and at most the %d classes", top_k, K2B200_MAX_TOP,
               rows->num_classes);
@@ -1154,10 +1157,13 @@ int32_t k2b200_token_scores_backward(const k2b200_class_rows *rows, const void *
                                      void *grad_scores, int64_t grad_outer_stride,
                                      int64_t grad_inner_stride, void *stream) {
   K2B_FORWARD(CheckRows(rows));
-  K2B_REQUIRE((uintptr_t)norm % 16 == 0, "norm that is not aligned to 16 bytes");
-  K2B_REQUIRE((uintptr_t)grad_scores % (rows->type == K2B200_F32 ? 4 : 2) == 0,
-              "a gradient that is not aligned to its type");
+  K2B_REQUIRE(Aligned(norm, 16), "norm that is not aligned to 16 bytes");
   K2B_REQUIRE(log_probs_grad && entropy_grad && top_log_probs_grad, "NULL pointer");
+  K2B_REQUIRE(Aligned(grad_scores, FloatSize(rows->type)) && Aligned(log_probs_grad->grad, 4) &&
+                  Aligned(entropy_grad->grad, 4) && Aligned(top_log_probs_grad->grad, 4),
+              "a gradient that is not aligned to its type");
+  K2B_REQUIRE(Aligned(tokens, IntSize(tokens_64)) && Aligned(top_tokens, 4),
+              "tokens that are not aligned to their type");
   K2B_REQUIRE(top_k >= 0 && top_k <= K2B200_MAX_TOP && top_k <= rows->num_classes,
               "top_k is %d: 0 to %d, and at most the %d classes", top_k, K2B200_MAX_TOP,
               rows->num_classes);

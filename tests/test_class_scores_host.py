@@ -103,6 +103,43 @@ def test_addresses_that_are_not_aligned_are_refused():
         assert status == INVALID and b"aligned" in _lib.lib.k2b200_last_error()
 
 
+def token_call(r, tokens=FAR, tokens_64=0, log_probs=FAR, entropy=None, top_values=FAR,
+               top_classes=FAR):
+    return _lib.lib.k2b200_token_scores(ctypes.byref(r), tokens, tokens_64, 2, log_probs, entropy,
+                                        top_values, top_classes, None, None)
+
+
+def token_backward_call(r, tokens=FAR, tokens_64=0, classes=FAR, ups=(FAR, FAR, FAR)):
+    a, b, c = (_lib.RowGrad(grad=up) for up in ups)
+    return _lib.lib.k2b200_token_scores_backward(
+        ctypes.byref(r), tokens, tokens_64, 2, classes, FAR, ctypes.byref(a), ctypes.byref(b),
+        ctypes.byref(c), FAR, 24, 8, None)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: token_scores(rows(lengths=FAR + 2)),
+    lambda: distil(rows(lengths=FAR + 4, lengths_64=1), teacher()),
+    lambda: token_call(rows(), tokens=FAR + 2), lambda: token_call(rows(), FAR + 4, 1),
+    lambda: token_call(rows(), log_probs=FAR + 2), lambda: token_call(rows(), entropy=FAR + 1),
+    lambda: token_call(rows(), top_values=FAR + 2), lambda: token_call(rows(), top_classes=FAR + 2),
+    lambda: token_backward_call(rows(), tokens=FAR + 4, tokens_64=1),
+    lambda: token_backward_call(rows(), classes=FAR + 2),
+    lambda: token_backward_call(rows(), ups=(FAR + 2, FAR, FAR)),
+    lambda: token_backward_call(rows(), ups=(FAR, FAR + 2, FAR)),
+    lambda: token_backward_call(rows(), ups=(FAR, FAR, FAR + 2)),
+    lambda: distil(rows(), teacher(tokens=FAR + 2)),
+    lambda: distil(rows(), teacher(tokens=FAR + 4, tokens_64=1)),
+    lambda: distil(rows(), teacher(scores=FAR + 2)),
+    lambda: distil_backward(rows(), teacher(scores=FAR + 1, type=2)),
+    lambda: distil(rows(), teacher(), loss=FAR + 2),
+    lambda: distil(rows(), teacher(), workspace=FAR + 4),
+    lambda: distil_backward(rows(), teacher(), workspace=FAR + 4),
+    lambda: distil_backward(rows(), teacher(), up=FAR + 2)])
+def test_arrays_that_are_not_aligned_are_refused(call):
+    """The device would stop at such an address."""
+    assert call() == INVALID and b"aligned" in _lib.lib.k2b200_last_error()
+
+
 def test_no_rows_are_no_work():
     empty = rows(outer=0, scores=None)
     assert token_scores(empty) == 0 and token_backward(empty) == 0
