@@ -488,6 +488,7 @@ at::Tensor DistillationLoss(const at::Tensor &scores, const at::Tensor &teacher_
   const at::Device device = scores.device();
   c10::cuda::CUDAGuard guard(device);
   RefuseForwardMode(scores);
+  RefuseForwardMode(teacher_log_probs);
   const bool graded = torch::autograd::compute_requires_grad(scores);
   at::Tensor loss, tokens, teacher_scores, workspace, norm, ready;
   RowsOf r;
