@@ -66,6 +66,7 @@ bool OneStride(const at::Tensor &t, int64_t from, int64_t to, int64_t *stride) {
   bool any = false;
   int64_t expect = 0;
   *stride = 0;
+  if (t.numel() == 0) return true;  // (nothing is read by it)
   for (int64_t d = to; d-- > from;) {
     if (t.size(d) == 1) continue;
     if (!any) {

@@ -22,3 +22,13 @@ def test_forward_mode_is_refused_wherever_it_comes_in():
                      lambda: k2.distillation_loss(x, tt, teacher)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("shape", [(5, 0, 7, 0, 9), (2, 0, 3, 0, 4, 9), (3, 5, 0, 7, 9), (0, 0, 9)])
+def test_no_rows_in_several_dimensions(shape):
+    x = torch.zeros(shape, device=DEV, requires_grad=True)
+    tt = torch.zeros(shape[:-1] + (3,), dtype=torch.int32, device=DEV)
+    outs = [k2.distillation_loss(x, tt, tt.float(), reduction=r) for r in ("none", "sum", "mean")]
+    got = k2.token_log_probs(x, tt[..., 0], top_k=2, entropy=True)
+    for out in outs + [got.log_probs, got.entropy, got.top_log_probs]:
+        assert torch.autograd.grad(out.sum(), x, retain_graph=True)[0].shape == shape
