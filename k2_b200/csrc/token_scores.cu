@@ -712,7 +712,7 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) four[g] = OrderOf(sums.group[g]);
           } else {
-            // (of 16 or 8 groups per lane four are made, or 8 for many classes)
+            // (16, 8 or 4 groups per lane become four; of 16 or 8 there are 8 for many classes)
 #pragma unroll
             for (int g = 0; g < 4; ++g) four[g] = 0;
 #pragma unroll
@@ -722,13 +722,13 @@ TokenRing(Rows<T> rows, TokenOut out, int32_t vectors, int32_t tiles) {
           if (top_k <= 16) {
             const uint32_t one[1] = {max(max(four[0], four[1]), max(four[2], four[3]))};
             bound = BoundOf(one, top_k);
-          } else if (kTeam == 32 || top_k <= 64) {
+          } else if (kTeam <= 128 || top_k <= 64) {
             bound = BoundOf(four, top_k);
-          } else {
+          } else if constexpr (kTeam > 128) {
             uint32_t eight[8] = {};
 #pragma unroll
             for (int g = 0; g < kTeam / 32; ++g)
-              eight[g & 7] = max(eight[g & 7], OrderOf(sh.group[kTeam == 32 ? 0 : 32 * g + lane]));
+              eight[g & 7] = max(eight[g & 7], OrderOf(sh.group[32 * g + lane]));
             bound = BoundOf(eight, top_k);
           }
           if (lane == 0) {

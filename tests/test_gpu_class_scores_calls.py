@@ -32,3 +32,16 @@ def test_no_rows_in_several_dimensions(shape):
     got = k2.token_log_probs(x, tt[..., 0], top_k=2, entropy=True)
     for out in outs + [got.log_probs, got.entropy, got.top_log_probs]:
         assert torch.autograd.grad(out.sum(), x, retain_graph=True)[0].shape == shape
+
+
+@pytest.mark.parametrize("rows,classes", [(300, 5000), (300, 20000), (2, 20000), (700, 5000)])
+def test_as_many_top_classes_as_a_block_has_threads_or_more(rows, classes):
+    """The bound comes from the groups that there are, and from those only: among scores around 0,
+    among log-probs, and where all scores are one very low value."""
+    g = torch.Generator(device=DEV).manual_seed(classes)
+    x = torch.randn(rows, classes, generator=g, device=DEV) * 3
+    for values in (x, torch.log_softmax(x, -1), x - 1e30):
+        order = torch.sort(values, dim=-1, descending=True, stable=True).indices.int()
+        for top_k in (63, 64, 65, 96, 113, 114, 127, 128):
+            got = k2.token_log_probs(values, top_k=top_k)
+            assert torch.equal(got.top_tokens, order[:, :top_k]), top_k
