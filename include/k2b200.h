@@ -42,12 +42,14 @@ typedef enum {
 
 /* Text of the last error on the calling thread. */
 const char *k2b200_last_error(void);
-/* ABI version of the library, bumped where a caller of the one before would break;
+/* ABI version of the library, bumped on any signature change (and up to 5 on any new entry point;
  * 3: pruned intersection, score derivatives, k2b200_upload_i32;
  * 4: k2b200_band_*;
- * 5: k2b200_peer_reduce_*, k2b200_loss_sum_all_reduce, zero_fill in k2b200_band_loss_args
- *    (k2b200_token_scores* and k2b200_distillation* came later and changed nothing else). */
+ * 5: k2b200_peer_reduce_*, k2b200_loss_sum_all_reduce, zero_fill in k2b200_band_loss_args). */
 int32_t k2b200_abi_version(void);
+/* Entry points that came within a version, bumped with each set of them and 0 in a new version; a
+ * library without this function has none (5.1: k2b200_token_scores*, k2b200_distillation*). */
+int32_t k2b200_abi_minor_version(void);
 
 /* Benchmark bookkeeping (no counterpart in the reference's bindings; its
  * benchmark harness, k2/csrc/benchmark/benchmark.h:49-66, times from outside).

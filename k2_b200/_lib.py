@@ -150,6 +150,7 @@ def _sig(name, restype, argtypes):
 
 _sig("k2b200_last_error", ctypes.c_char_p, [])
 _sig("k2b200_abi_version", c_i32, [])
+_sig("k2b200_abi_minor_version", c_i32, [])
 _sig("k2b200_kernel_launch_count", c_i64, [])
 _sig("k2b200_profile_enable", None, [c_i32])
 _sig("k2b200_profile_kernel", ctypes.c_char_p, [c_i32])
@@ -303,7 +304,8 @@ _sig("k2b200_distillation_backward", c_i32,
       c_vp, c_i64, c_i64, c_vp, c_sz, c_vp])
 
 EXPORTED = [
-    "k2b200_last_error", "k2b200_abi_version", "k2b200_kernel_launch_count",
+    "k2b200_last_error", "k2b200_abi_version", "k2b200_abi_minor_version",
+    "k2b200_kernel_launch_count",
     "k2b200_profile_enable", "k2b200_profile_kernel", "k2b200_profile_read_ms", "k2b200_row_splits_to_row_ids",
     "k2b200_upload_i32",
     "k2b200_exclusive_sum_tmp_bytes", "k2b200_exclusive_sum",

@@ -445,6 +445,7 @@ extern "C" {
 
 const char *k2b200_last_error(void) { return LastError(); }
 int32_t k2b200_abi_version(void) { return 5; }
+int32_t k2b200_abi_minor_version(void) { return 1; }
 int64_t k2b200_kernel_launch_count(void) { return LaunchCount(); }
 void k2b200_profile_enable(int32_t on) { SetProfiling(on != 0); }
 const char *k2b200_profile_kernel(int32_t phase) { return PhaseKernel(phase); }

@@ -146,6 +146,11 @@ def test_no_rows_are_no_work():
     assert distil_backward(empty, teacher()) == 0
 
 
+def test_a_host_can_ask_whether_they_are_there():
+    """A library of the same version that came before them has no minor version."""
+    assert (_lib.lib.k2b200_abi_version(), _lib.lib.k2b200_abi_minor_version()) >= (5, 1)
+
+
 def test_there_is_no_cpu_path():
     x, token = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="CUDA tensor"):
