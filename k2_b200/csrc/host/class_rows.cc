@@ -4,6 +4,7 @@
 #include "class_rows.h"
 
 #include <ATen/SavedTensorHooks.h>
+#include <ATen/core/DimVector.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -95,7 +96,7 @@ class Saved {
  public:
   void Keep(const at::Tensor &t) {
     variable_ = SavedVariable(t, false);
-    sizes_ = t.sizes().vec();
+    sizes_ = at::DimVector(t.sizes());
     type_ = t.scalar_type();
     device_ = t.device();
     there_ = true;
@@ -104,7 +105,7 @@ class Saved {
   at::Device device() const { return device_; }
   at::Tensor Get() const {
     const at::Tensor t = variable_.unpack();
-    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.sizes() == sizes_ &&
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.sizes() == at::IntArrayRef(sizes_) &&
                     t.scalar_type() == type_ && t.device() == device_,
                 "hooks gave back a saved tensor of other sizes, type or device than they got");
     return t;
@@ -113,7 +114,7 @@ class Saved {
 
  private:
   SavedVariable variable_;
-  std::vector<int64_t> sizes_;
+  at::DimVector sizes_;
   at::ScalarType type_ = at::kFloat;
   at::Device device_ = at::kCPU;
   bool there_ = false;
