@@ -95,7 +95,8 @@ at::Tensor Plain(const at::Tensor &t) { return (t.is_neg() ? t.resolve_neg() : t
 class Saved {
  public:
   void Keep(const at::Tensor &t) {
-    variable_ = SavedVariable(t, false);
+    // (a teacher's of inference mode have no version that torch could compare: a copy)
+    variable_ = SavedVariable(t.is_inference() ? t.clone() : t, false);
     sizes_ = at::DimVector(t.sizes());
     type_ = t.scalar_type();
     device_ = t.device();

@@ -204,3 +204,30 @@ def test_what_a_hook_raises_arrives(kind):
         out = call(kind, x, d, d["lengths"])
     with pytest.raises(Stop):
         torch.autograd.grad(out, x)
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_a_teacher_in_inference_mode(reduction):
+    """Its tensors have no versions that could be compared: they are copied."""
+    g = torch.Generator().manual_seed(0)
+    of_teacher = torch.randn(*SHAPE, 60, generator=g).to(DEV)
+    x = torch.randn(*SHAPE, 60, generator=g).to(DEV).requires_grad_(True)
+    with torch.inference_mode():
+        lengths = torch.tensor([5, 2, 4], device=DEV)
+        named = k2.token_log_probs(of_teacher, top_k=8, lengths=lengths)
+    loss = k2.distillation_loss(x, named.top_tokens, named.top_log_probs, reduction=reduction,
+                                lengths=lengths)
+    scored = k2.token_log_probs(x, named.top_tokens[..., 0], lengths=lengths)
+    want, tol = distil_reference(x.detach(), named.top_tokens, named.top_log_probs, 1.0, 1.0,
+                                 reduction, live(lengths))
+    up = dict(log_probs=torch.ones(SHAPE))
+    given, given_tol = tokens_reference(x.detach(), named.top_tokens[..., 0].clone(), 0,
+                                        live(lengths), up)
+    with torch.inference_mode():
+        named.top_tokens.zero_()
+        named.top_log_probs.zero_()
+        lengths.zero_()
+    grad, = torch.autograd.grad(loss.sum(), x)
+    assert_close(grad, want["grad"], tol["grad"])
+    grad, = torch.autograd.grad(scored.log_probs.sum(), x)
+    assert_close(grad, given["grad"], given_tol["grad"])
