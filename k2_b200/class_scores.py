@@ -34,7 +34,8 @@ def token_log_probs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         log-prob is 0 and has no gradient.  Any other number that is no class gives NaN, in the
         log-prob and, where that has an upstream gradient, in the row's gradient.
       top_k: so many of the largest log-probs, and their classes (0 to 128); among equal logits
-        the lowest class comes first.
+        the lowest class comes first.  A short row's time grows steeply above 32 (64000 rows of
+        500 classes: 57 us for 8, 122 for 32, 629 for 64, 858 for 128).
       entropy: whether -sum_c p_c log p_c is wanted.
       lengths: [N] int32 or int64, on the CPU or the device, for logits [N, T, C]: frames from
         `lengths[n]` on are not read; they get 0 everywhere, -1 as top classes, and no
@@ -74,7 +75,9 @@ def distillation_loss(logits: torch.Tensor, teacher_tokens: torch.Tensor,
 
     With "sum" and "mean" the gradient is made beside the loss, while a row is at hand, for an
     upstream of 1, and made again from the logits where the upstream is another: a factor of the
-    loss is cheaper as `weight` than as a product."""
+    loss is cheaper as `weight` than as a product.  It takes as much memory as the logits until the
+    backward pass; under `torch.autograd.graph.saved_tensors_hooks` (offloading, checkpoints) it
+    is made there."""
     return _host.distillation_loss(logits, teacher_tokens, teacher_log_probs, temperature, weight,
                                    reduction, lengths)
 

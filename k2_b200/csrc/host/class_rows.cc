@@ -130,6 +130,8 @@ struct RowsOf {
 };
 
 // Scores of adjacent classes whose rows lie at two strides are read in place, others are copied.
+// (what is refused here, with Python's lock held, cannot come up in a backward pass, which has no such
+// lock: Saved gives back sizes, types and devices that have been through here)
 RowsOf MakeRows(const at::Tensor &scores, const c10::optional<at::Tensor> &lengths) {
   RequireCuda(scores, "logits");
   Require(scores.dim() >= 1 && FloatType(scores) >= 0,
